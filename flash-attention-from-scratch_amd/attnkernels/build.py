@@ -33,7 +33,8 @@ LIB = PKG / "libattnkernels.so"
 EXT_NAME = "attnkernels_ext"
 ARCH = os.environ.get("ATTN_OFFLOAD_ARCH", "gfx950")
 
-HIP_SOURCES = ["prefill.hip", "decode.hip", "cache_write.hip", "stream.hip"]
+HIP_SOURCES = ["prefill.hip", "decode.hip", "cache_write.hip", "stream.hip", "cache_mxfp4.hip",
+               "decode_mx.hip", "prompt_weights.hip", "evict.hip"]
 CPP_SOURCES = ["capi.cpp"]
 
 # Packed FP32 VALU ops stay disabled on this pool; hipcc's host pass warns it

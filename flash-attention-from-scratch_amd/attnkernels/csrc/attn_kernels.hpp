@@ -70,6 +70,88 @@ struct CacheWriteArgs {
     void* stream;
 };
 
+// Rows of the 4-bit paged cache (mxfp4.hpp), written from key and value or read
+// into key_out and value_out.
+struct CacheMxArgs {
+    const void* key;        // [num_tokens, hkv, head_dim] fp16 or bf16, token stride key_stride elements
+    const void* value;
+    void* key_out;          // [num_tokens, hkv, head_dim], contiguous
+    void* value_out;
+    void* k_codes;          // [num_blocks, hkv, bs, head_dim / 2] bytes
+    void* k_scales;         // [num_blocks, hkv, bs, head_dim / 32] bytes
+    void* v_codes;
+    void* v_scales;
+    const int64_t* slots;   // [num_tokens]
+    int64_t num_tokens, hkv, head_dim, num_blocks, bs;  // head_dim a multiple of 32
+    int64_t key_stride, value_stride;  // multiples of 8
+    bool bf16;
+    void* stream;
+};
+
+// Decode over a 4-bit cache, or over an fp16 or bf16 one, with the attention
+// weights added to a sum per token (weights, or nullptr: not).
+struct DecodeMxArgs {
+    const void* q;         // [B, hq, D] fp16 or bf16
+    const void* k;         // rows [num_blocks, hkv, bs, ...]: codes of D / 2 bytes, or D elements of q's type
+    const void* v;
+    const void* k_scales;  // [num_blocks, hkv, bs, D / 32] bytes; nullptr: k and v hold elements of q's type
+    const void* v_scales;
+    const int32_t* block_tables;  // [B, max_blocks]
+    const int32_t* context_lens;  // [B]
+    void* out;             // [B, hq, D], q's type
+    float* o_part;         // [B, hq, S, D]  split partials
+    float* m_part;         // [B, hq, S]
+    float* l_part;         // [B, hq, S]
+    float* scores;         // [B, hq, scores_stride]: scale * log2(e) * q.k, where weights are wanted
+    float* weights;        // [B, hkv, >= max_ctx], strides in elements below
+    int32_t* counters;     // one per (sequence, kv head), zero on entry and left zero
+    int64_t batch, hq, hkv, d, num_blocks, bs, max_blocks, max_ctx, partition, num_splits;
+    int64_t scores_stride, w_stride_b, w_stride_h;
+    bool bf16;
+    float sl2;             // scale * log2(e)
+    void* stream;
+};
+
+hipError_t cache_write_mxfp4_launch(const CacheMxArgs& a);
+hipError_t cache_read_mxfp4_launch(const CacheMxArgs& a);
+hipError_t decode_mx_launch(const DecodeMxArgs& a);
+// Tokens per split where the caller leaves them to the library: a multiple of 256.
+int64_t decode_mx_partition(int64_t batch, int64_t hkv, int64_t max_ctx);
+
+// Eviction by accumulated weight (evict.hip).
+struct EvictArgs {
+    void* rows[4];          // K, V and (4-bit cache) their scales: [num_blocks, hkv, bs, row_bytes[i]]; nullptr ends them
+    int64_t row_bytes[4];   // K and V: multiples of 16
+    const int32_t* block_tables;      // [B, max_blocks]
+    const int32_t* new_block_tables;  // [B, new_max_blocks] pages that kept rows are written to; nullptr: their own
+    const int32_t* context_lens;      // [B]
+    const float* weights;   // [B, hkv, length], strides in elements below
+    int32_t* new_lens;      // [B]
+    float* new_weights;     // [B, hkv, length]
+    int32_t* kept;          // [B, hkv, budget]
+    int64_t w_stride_b, w_stride_h;
+    int64_t batch, hkv, num_blocks, bs, max_blocks, new_max_blocks, length, budget, recent;  // 0 <= recent <= budget
+    void* stream;
+};
+hipError_t evict_launch(const EvictArgs& a);
+
+// Attention weights of a prompt's queries, summed per token (prompt_weights.hip).
+struct PromptWeightsArgs {
+    const void* q;          // [total, hq, d] fp16 or bf16, token stride q_stride elements
+    const void* k;          // [total, hkv, d], token stride k_stride
+    const int32_t* cu;      // [batch + 1] sequence starts
+    float* weights;         // [batch, hkv, length], strides in elements below
+    void* workspace;
+    int64_t batch, total, hq, hkv, d, max_seqlen, last, length;
+    int64_t q_stride, k_stride, w_stride_b, w_stride_h;
+    bool bf16;
+    float sl2;              // scale * log2(e)
+    void* stream;
+};
+hipError_t prompt_weights_launch(const PromptWeightsArgs& a);
+size_t prompt_weights_workspace(int64_t batch, int64_t total, int64_t hq, int64_t hkv, int64_t max_seqlen,
+                                int64_t last);
+
 hipError_t prefill_launch(const PrefillArgs& a);
 hipError_t decode_launch(const DecodeArgs& a);
 

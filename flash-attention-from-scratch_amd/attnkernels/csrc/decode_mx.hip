@@ -1,0 +1,537 @@
+// Decode attention (one query token per sequence) over the 4-bit paged cache
+// (MXFP4, mxfp4.hpp) and, where attention weights are summed per cached token,
+// over fp16 and bf16 caches too.  Not in the reference, whose decode
+// (attnkernels/csrc/paged_decode.cu) reads an fp16 cache and keeps no weights.
+//
+//   s_t = scale q.k_t,  p = softmax(s),  o = sum_t p_t v_t      per query head
+//   weights[b, kv head, t] += sum over the kv head's G query heads of p_t
+//
+// Bound by memory: 2 (D/2 + D/32) bytes a token and kv head in 4 bits (136 at
+// D = 128, against 512 in fp16), 8 more for the weights.  Both products run on
+// 16x16x32 MFMAs with the head group padded to 16 rows, for every G up to 16:
+// the matrix cores have the time, and the vector work per byte does not grow
+// with G.
+//   * A wave takes 32 tokens per iteration, two blocks of 16.  S^T = K Q^T: lane
+//     (n = l%16, g = l/16) holds token n of a block and D/4 of its channels.
+//     In 4 bits that is one scale group (D = 128) or half of one (D = 64), so a
+//     lane's codes have one scale, and the hardware's conversions turn a dword
+//     of codes into the eight values of an operand in four instructions.
+//   * The lane then holds the scores of query head n for tokens 4g..4g+3 of both
+//     blocks, which is P as the operand of O += P V once rounded.  V's operand
+//     for column n is the D/16 channels D/16 n.. of those eight tokens: the lane
+//     loads them row by row and pairs the tokens with v_perm.
+//   * exp2 against a reference maximum that moves only when a score exceeds it
+//     by more than 8, sums in fp32.
+// With weights, the scores (scale * log2 e * q.k in fp32) go to a workspace, and
+// a second kernel, which knows every split's maximum and sum, turns them into
+// weights while it merges the splits' outputs.
+#include <algorithm>
+
+#include "attn_kernels.hpp"
+#include "index_math.hpp"
+#include "mxfp4.hpp"
+
+namespace ak {
+
+namespace {
+
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kTile = 32;           // tokens per wave iteration
+constexpr int kMaxGroup = 16;       // query heads per kv head: rows of the MFMA
+constexpr int kFinishTokens = 1024; // tokens per workgroup of the finishing kernel
+constexpr float kLowest = -3.402823466e38f;
+
+struct Params {
+    const void *q, *k, *v;
+    const uint8_t *k_scales, *v_scales;
+    const int *block_tables, *ctx_lens;
+    void* out;
+    float *o_part, *m_part, *l_part, *scores, *weights;
+    int32_t* counters;
+    int64_t scores_stride, w_stride_b, w_stride_h;
+    int hkv, group, bs, bs_shift, max_blocks, num_blocks, max_tok, partition, num_splits;
+    float sl2;
+};
+
+__device__ __forceinline__ void coherent_store(float* p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float coherent_load(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, kWave));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) x += __shfl_xor(x, m, kWave);
+    return x;
+}
+
+// The running maximum m and sum l of one query row over its ns splits, by one
+// wave: split s starts at mp[s], lp[s].  Splits without weight (l = 0) count
+// nothing; a row without any has l = 0.
+__device__ __forceinline__ void merge_stats(const float* mp, const float* lp, int ns, int lane, float& m, float& l) {
+    float M = kLowest, L = 0.f;
+    for (int s = lane; s < ns; s += kWave) {
+        const float ls = coherent_load(lp + s), ms = ls == 0.f ? kLowest : coherent_load(mp + s);
+        const float mn = fmaxf(M, ms);
+        L = L * exp2_fast(M - mn) + ls * exp2_fast(ms - mn);
+        M = mn;
+    }
+    m = wave_max(M);
+    l = wave_sum(L * exp2_fast(M - m));
+}
+
+// Head `head`'s output row from its ns split partials, by `threads` threads of
+// which this is tid: 4 channels each and every SG-th split, joined through LDS.
+template <int D, class T>
+__device__ __forceinline__ void merge_row(const Params& a, size_t row, int ns, float m, float l, int tid) {
+    constexpr int UNITS = D / 4, SG = kThreads / UNITS;
+    __shared__ f32x4 part[kThreads];
+    const int u = tid % UNITS, sg = tid / UNITS;
+    const float* mp = a.m_part + row * a.num_splits;
+    const float* lp = a.l_part + row * a.num_splits;
+    const float* op = a.o_part + (row * a.num_splits) * D + u * 4;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = sg; s < ns; s += SG) {
+        const float ls = coherent_load(lp + s);
+        if (ls == 0.f) continue;
+        const float w = ls * exp2_fast(coherent_load(mp + s) - m) * inv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += w * coherent_load(op + (size_t)s * D + i);
+    }
+    __syncthreads();  // a row before this one may still be read
+    part[tid] = o;
+    __syncthreads();
+    if (sg == 0) {
+#pragma unroll
+        for (int k = 1; k < SG; ++k) o += part[k * UNITS + u];
+        uint32_t* dst = static_cast<uint32_t*>(a.out) + (row * D + u * 4) / 2;
+        dst[0] = Half<T>::pack(o[0], o[1]);
+        dst[1] = Half<T>::pack(o[2], o[3]);
+    }
+}
+
+// Where a lane's tokens are read: pages of the tile's tokens, one per lane (token
+// t + lane % 32), -1 where there is none.
+__device__ __forceinline__ int page_index(int t, const Params& a) {
+    return a.bs_shift >= 0 ? t >> a.bs_shift : t / a.bs;
+}
+
+template <int D, class T, bool MX>
+struct Tile {
+    static constexpr int KW = MX ? D / 32 : D / 8;    // dwords of K per block: a quarter row
+    static constexpr int VW = MX ? 1 : D / 32;        // dwords of a V row's D/16 channels (4 bits, D = 64: half of one)
+    uint32_t k[2][KW], v[2][4][VW];
+    uint32_t ks[2], vs[2][4];
+    uint32_t valid;                                   // bit i: token t + i is read (wave-uniform)
+};
+
+template <int D, class T, bool MX, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads) decode_mx_kernel(const Params a) {
+    using Tl = Tile<D, T, MX>;
+    constexpr int DPL = D / 16;             // channels of a V row per lane = products per tile
+    constexpr int KS = D / 32;              // products of S^T per block
+    constexpr int KROW = MX ? D / 2 : 2 * D;  // bytes
+    constexpr float kShift = 7.f, kPMax = 32768.f;
+    __shared__ float red_acc[kWaves][kMaxGroup][D];
+    __shared__ float red_m[kWaves][kMaxGroup], red_l[kWaves][kMaxGroup];
+    __shared__ int last;
+
+    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
+    const int G = a.group, hq = a.hkv * G;
+    const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int ctx = min(a.ctx_lens[b], a.max_tok);
+    const int start = split * a.partition, end = min(ctx, start + a.partition);
+    const size_t row0 = (size_t)b * hq + (size_t)kvh * G;
+    const int ns = ctx > 0 ? (ctx + a.partition - 1) / a.partition : 0;
+    const bool direct = !WEIGHTS && (a.num_splits == 1 || (a.counters && ns <= 1));
+    if (start >= end) {
+        if (direct && split == 0)
+            for (int i = tid; i < G * D / 2; i += kThreads) static_cast<uint32_t*>(a.out)[row0 * (D / 2) + i] = 0;
+        return;
+    }
+    const int* bt = a.block_tables + (size_t)b * a.max_blocks;
+    const int stride = kWaves * kTile;
+    int t = start + w * kTile;
+
+    auto pages = [&](int tile) {  // the page of token tile + lane % 32
+        const int tok = tile + (lane & 31);
+        return tok < end ? bt[page_index(tok, a)] : -1;
+    };
+    const bool fast_bs = a.bs % 16 == 0;
+
+    // Q^T: head n (zeros past the group), the channels that the lane's K holds.
+    u32x4 qf[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+        qf[i] = u32x4{0, 0, 0, 0};
+        if (n < G) {
+            const int ch = MX ? (D / 4) * g + 8 * i : 32 * i + 8 * g;
+            qf[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + (row0 + n) * D + ch);
+        }
+    }
+
+    // Loads of one lane from the row of a token (row: counted over the pool).
+    auto load_k = [&](Tl& x, int blk, size_t row) {
+        const char* p = static_cast<const char*>(a.k) + row * KROW;
+        if constexpr (MX && D == 128) {
+            const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 16 * g));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.k[blk][i] = y[i];
+        } else if constexpr (MX) {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + 8 * g));
+            x.k[blk][0] = y[0];
+            x.k[blk][1] = y[1];
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 64 * s + 16 * g));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x.k[blk][4 * s + i] = y[i];
+            }
+        }
+        if constexpr (MX) x.ks[blk] = a.k_scales[row * (D / 32) + (D == 128 ? g : g / 2)];
+    };
+    auto load_v = [&](Tl& x, int blk, int r, size_t row) {
+        const char* p = static_cast<const char*>(a.v) + row * KROW;
+        if constexpr (MX && D == 128) {
+            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p + 4 * n));
+        } else if constexpr (MX) {
+            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p + 2 * n));
+        } else {
+            typedef uint32_t vec __attribute__((ext_vector_type(Tl::VW)));
+            const vec y = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p + 4 * Tl::VW * n));
+#pragma unroll
+            for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = y[i];
+        }
+        if constexpr (MX) x.vs[blk][r] = a.v_scales[row * (D / 32) + n / 8 * (D / 64) + (D == 128 ? n / 4 % 2 : 0)];
+    };
+    auto load = [&](Tl& x, int tile, int pid) {
+        x.valid = (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)pid < (unsigned)a.num_blocks);
+        if (fast_bs && x.valid == 0xffffffffu) {
+            // Each block within one page: two page ids for the wave.
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                const int p = __builtin_amdgcn_readlane(pid, 16 * blk), tb = uniform(tile) + 16 * blk;
+                const int in = a.bs_shift >= 0 ? tb & (a.bs - 1) : tb % a.bs;
+                const size_t row = ((size_t)p * a.hkv + kvh) * a.bs + in;
+                load_k(x, blk, row + n);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) load_v(x, blk, r, row + 4 * g + r);
+            }
+        } else {
+            // Every token's row on its own, as lane (token % 32) knows it; rows
+            // that are not read are zeros.
+            const int tok = tile + (lane & 31);
+            const int in = a.bs_shift >= 0 ? tok & (a.bs - 1) : tok % a.bs;
+            auto row_of = [&](int i) {
+                const int p = __shfl(pid, i, kWave), o = __shfl(in, i, kWave);
+                return ((size_t)p * a.hkv + kvh) * a.bs + o;
+            };
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                x.ks[blk] = 127;
+#pragma unroll
+                for (int i = 0; i < Tl::KW; ++i) x.k[blk][i] = 0;
+                const size_t kr = row_of(16 * blk + n);
+                if (x.valid >> (16 * blk + n) & 1) load_k(x, blk, kr);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x.vs[blk][r] = 127;
+#pragma unroll
+                    for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = 0;
+                    const size_t vr = row_of(16 * blk + 4 * g + r);
+                    if (x.valid >> (16 * blk + 4 * g + r) & 1) load_v(x, blk, r, vr);
+                }
+            }
+        }
+    };
+
+    // Reference maximum of head n (the same in its four lanes), this lane's
+    // share of l, and acc[j][r]: head 4g + r, channel DPL n + j.
+    float m_own = kLowest, l_own = 0.f;
+    f32x4 acc[DPL];
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float* scores = WEIGHTS ? a.scores + (row0 + (n < G ? n : 0)) * a.scores_stride + 4 * g : nullptr;
+
+    auto step = [&](const Tl& x, int tile) {
+        f32x4 s[2];
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            s[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                u32x4 kf;
+                if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], mx_scale(x.ks[blk]));
+                else kf = u32x4{x.k[blk][4 * i], x.k[blk][4 * i + 1], x.k[blk][4 * i + 2], x.k[blk][4 * i + 3]};
+                s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[blk][r] *= a.sl2;
+            if (x.valid != 0xffffffffu) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    s[blk][r] = x.valid >> (16 * blk + 4 * g + r) & 1 ? s[blk][r] : -INFINITY;
+            }
+            if constexpr (WEIGHTS) {
+                if (n < G) *reinterpret_cast<f32x4*>(scores + tile + 16 * blk) = s[blk];
+            }
+        }
+        float p[8];
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+            ok = ok && p[i] <= kPMax;
+        }
+        if (__builtin_amdgcn_ballot_w64(!ok)) {
+            // Move the reference maximum of every head to its running maximum.
+            float mx = m_own;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+            const float alpha = exp2_fast(m_own - mx);
+            l_own *= alpha;
+            m_own = mx;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {  // accumulator row r is head 4g + r
+                const float al = __shfl(alpha, 4 * g + r, kWave);
+#pragma unroll
+                for (int j = 0; j < DPL; ++j) acc[j][r] *= al;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+        }
+        l_own += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        u32x4 pf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pf[i] = Half<T>::pack(p[2 * i], p[2 * i + 1]);
+        // V: the lane's channels of its eight tokens, two tokens to a register.
+        uint32_t vr[8][DPL / 2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (MX) {
+                const float sc = mx_scale(x.vs[i / 4][i % 4]);
+                const uint32_t c = x.v[i / 4][i % 4][0];
+                vr[i][0] = Half<T>::template decode<0>(c, sc);
+                vr[i][1] = Half<T>::template decode<1>(c, sc);
+                if constexpr (DPL == 8) {
+                    vr[i][2] = Half<T>::template decode<2>(c, sc);
+                    vr[i][3] = Half<T>::template decode<3>(c, sc);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < DPL / 2; ++j) vr[i][j] = x.v[i / 4][i % 4][j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) {
+            const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+            u32x4 f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][j / 2], vr[2 * i][j / 2], sel);
+            acc[j] = Half<T>::mfma(pf, f, acc[j]);
+        }
+    };
+
+    if (t < end) {
+        int pid = pages(t), next = pages(t + stride);
+        if constexpr (MX) {  // the next tile's rows are on their way while this one is computed
+            Tl x, y;
+            load(x, t, pid);
+            while (true) {
+                const int t1 = t + stride, t2 = t1 + stride;
+                pid = pages(t2);
+                if (t1 < end) load(y, t1, next);
+                step(x, t);
+                if (t1 >= end) break;
+                next = pages(t2 + stride);
+                if (t2 < end) load(x, t2, pid);
+                step(y, t1);
+                if (t2 >= end) break;
+                t = t2;
+            }
+        } else {
+            for (; t < end; t += stride) {
+                Tl x;
+                load(x, t, pid);
+                pid = next;
+                next = pages(t + 2 * stride);
+                step(x, t);
+            }
+        }
+    }
+
+    // Merge: l over the four lanes of each head, then the waves through LDS.
+    l_own += __shfl_xor(l_own, 16, kWave);
+    l_own += __shfl_xor(l_own, 32, kWave);
+    if (g == 0) {
+        red_m[w][n] = m_own;
+        red_l[w][n] = l_own;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (4 * g + r < G) {
+#pragma unroll
+            for (int j = 0; j < DPL; ++j) red_acc[w][4 * g + r][DPL * n + j] = acc[j][r];
+        }
+    __syncthreads();
+    const bool fused = !WEIGHTS && a.counters && !direct;
+    for (int i = tid; i < G * D / 2; i += kThreads) {
+        const int h = i / (D / 2), d = 2 * (i % (D / 2));
+        float M = red_m[0][h];
+#pragma unroll
+        for (int v = 1; v < kWaves; ++v) M = fmaxf(M, red_m[v][h]);
+        float L = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+            const float wv = exp2_fast(red_m[v][h] - M);
+            L += red_l[v][h] * wv;
+            o0 += red_acc[v][h][d] * wv;
+            o1 += red_acc[v][h][d + 1] * wv;
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;  // no token that counts: zeros
+        const size_t slot = (row0 + h) * a.num_splits + split;
+        if (direct) {
+            static_cast<uint32_t*>(a.out)[((row0 + h) * D + d) / 2] = Half<T>::pack(o0 * inv, o1 * inv);
+        } else {
+            coherent_store(a.o_part + slot * D + d, o0 * inv);
+            coherent_store(a.o_part + slot * D + d + 1, o1 * inv);
+            if (d == 0) {
+                coherent_store(a.m_part + slot, M);
+                coherent_store(a.l_part + slot, L * (1.f / 128.f));  // without the shift of P
+            }
+        }
+    }
+    if (!fused) return;
+    // The last split of the sequence and kv head to finish merges them all.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int32_t* cnt = a.counters + (size_t)b * a.hkv + kvh;
+    if (tid == 0) last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
+    __syncthreads();
+    if (!last) return;
+    if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int h = w; h < G; h += kWaves) {
+        float m, l;
+        merge_stats(a.m_part + (row0 + h) * a.num_splits, a.l_part + (row0 + h) * a.num_splits, ns, lane, m, l);
+        if (lane == 0) {
+            red_m[0][h] = m;
+            red_l[0][h] = l;
+        }
+    }
+    __syncthreads();
+    for (int h = 0; h < G; ++h) merge_row<D, T>(a, row0 + h, ns, red_m[0][h], red_l[0][h], tid);
+}
+
+// After decode_mx_kernel: merges the splits' outputs, and turns the scores into
+// weights.  Workgroup c of a (kv head, sequence) has tokens c * kFinishTokens on
+// and the heads h with h % (workgroups with tokens) == c.
+template <int D, class T, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads) decode_mx_finish_kernel(const Params a) {
+    __shared__ float row_m[kMaxGroup], row_l[kMaxGroup];
+    const int c = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const int G = a.group, hq = a.hkv * G;
+    const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+    const int ctx = max(min(a.ctx_lens[b], a.max_tok), 0);
+    const size_t row0 = (size_t)b * hq + (size_t)kvh * G;
+    const int ns = (ctx + a.partition - 1) / a.partition;
+    const int active = WEIGHTS ? max((ctx + kFinishTokens - 1) / kFinishTokens, 1) : gridDim.x;
+    if (c >= active) return;
+    for (int h = w; h < G; h += kWaves) {
+        float m, l;
+        merge_stats(a.m_part + (row0 + h) * a.num_splits, a.l_part + (row0 + h) * a.num_splits, ns, lane, m, l);
+        if (lane == 0) {
+            row_m[h] = m;
+            row_l[h] = l;
+        }
+    }
+    __syncthreads();
+    if constexpr (WEIGHTS) {
+        float* wt = a.weights + b * a.w_stride_b + kvh * a.w_stride_h;
+        const int t0 = c * kFinishTokens, t1 = min(ctx, t0 + kFinishTokens);
+        for (int t = t0 + tid; t < t1; t += kThreads) {
+            const float* s = a.scores + row0 * a.scores_stride + t;
+            float sum = 0.f;
+            for (int h = 0; h < G; ++h) {
+                const float l = row_l[h];
+                if (l != 0.f) sum += exp2_fast(s[h * a.scores_stride] - row_m[h]) * (1.f / l);
+            }
+            wt[t] += sum;
+        }
+    }
+    for (int h = c; h < G; h += active) merge_row<D, T>(a, row0 + h, ns, row_m[h], row_l[h], tid);
+}
+
+template <int D, class T, bool MX, bool WEIGHTS>
+hipError_t launch(const DecodeMxArgs& x) {
+    Params p{};
+    p.q = x.q;
+    p.k = x.k;
+    p.v = x.v;
+    p.k_scales = static_cast<const uint8_t*>(x.k_scales);
+    p.v_scales = static_cast<const uint8_t*>(x.v_scales);
+    p.block_tables = x.block_tables;
+    p.ctx_lens = x.context_lens;
+    p.out = x.out;
+    p.o_part = x.o_part;
+    p.m_part = x.m_part;
+    p.l_part = x.l_part;
+    p.scores = x.scores;
+    p.weights = x.weights;
+    p.scores_stride = x.scores_stride;
+    p.w_stride_b = x.w_stride_b;
+    p.w_stride_h = x.w_stride_h;
+    p.hkv = (int)x.hkv;
+    p.group = (int)(x.hq / x.hkv);
+    p.bs = (int)x.bs;
+    p.bs_shift = (x.bs & (x.bs - 1)) == 0 ? __builtin_ctzll((unsigned long long)x.bs) : -1;
+    p.max_blocks = (int)x.max_blocks;
+    p.num_blocks = (int)x.num_blocks;
+    p.max_tok = (int)std::min(x.max_blocks * x.bs, x.max_ctx);
+    p.partition = (int)x.partition;
+    p.num_splits = (int)x.num_splits;
+    p.sl2 = x.sl2;
+    const bool merge_here = !WEIGHTS && x.num_splits <= kFusedMaxSplits;
+    p.counters = merge_here ? x.counters : nullptr;
+    const dim3 grid((unsigned)x.hkv, (unsigned)x.num_splits, (unsigned)x.batch);
+    hipLaunchKernelGGL((decode_mx_kernel<D, T, MX, WEIGHTS>), grid, dim3(kThreads), 0, (hipStream_t)x.stream, p);
+    if (merge_here && (x.num_splits == 1 || x.counters)) return hipGetLastError();
+    const unsigned chunks = WEIGHTS ? (unsigned)((p.max_tok + kFinishTokens - 1) / kFinishTokens) : (unsigned)p.group;
+    hipLaunchKernelGGL((decode_mx_finish_kernel<D, T, WEIGHTS>), dim3(chunks, (unsigned)x.hkv, (unsigned)x.batch),
+                       dim3(kThreads), 0, (hipStream_t)x.stream, p);
+    return hipGetLastError();
+}
+
+template <int D, class T>
+hipError_t launch_typed(const DecodeMxArgs& x) {
+    if (!x.k_scales) return launch<D, T, false, true>(x);  // without weights a full-precision cache is paged_decode's
+    return x.weights ? launch<D, T, true, true>(x) : launch<D, T, true, false>(x);
+}
+
+}  // namespace
+
+// About four workgroups for each of the 256 CUs.
+int64_t decode_mx_partition(int64_t batch, int64_t hkv, int64_t max_ctx) {
+    constexpr int64_t kChunk = 256, kWorkgroups = 1024;
+    const int64_t chunks = (max_ctx + kChunk - 1) / kChunk;
+    const int64_t splits = std::min(chunks, (kWorkgroups + batch * hkv - 1) / (batch * hkv));
+    return (chunks + splits - 1) / splits * kChunk;
+}
+
+hipError_t decode_mx_launch(const DecodeMxArgs& x) {
+    if (x.d == 128) return x.bf16 ? launch_typed<128, bf16>(x) : launch_typed<128, f16>(x);
+    return x.bf16 ? launch_typed<64, bf16>(x) : launch_typed<64, f16>(x);
+}
+
+}  // namespace ak

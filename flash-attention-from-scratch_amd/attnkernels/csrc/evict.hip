@@ -1,0 +1,270 @@
+// Eviction from the paged KV cache by accumulated attention weight: of every
+// sequence longer than a budget, each kv head keeps its last `recent` tokens and
+// the others of the largest weight, and the kept rows move to the front of the
+// sequence's pages in their order.  Not in the reference, which has no cache
+// upkeep.
+//
+// evict_select_kernel, one workgroup per (sequence, kv head), bound by latency:
+// the weights as integers that order as they do; a radix select from the top
+// bits down finds the key of the last one kept (LDS histograms of 2048 bins,
+// three passes); then one pass in order of position counts those above it and
+// those equal to it before each token (ties go to the lowest positions), which
+// is its new position.
+//
+// evict_move_kernel, bound by memory: rows of the kept tokens are read and
+// written once.  In place, row i becomes what row kept[i] >= i was: a workgroup
+// owns a column of up to 128 bytes of one head's rows, so that no other touches
+// its bytes, reads a batch of rows, waits until all of it is read, and writes it.
+// Later batches only read rows behind what has been written, so nothing else
+// has to be ordered.
+#include <algorithm>
+
+#include "attn_kernels.hpp"
+#include "wave.hpp"
+
+namespace ak {
+
+namespace {
+
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
+constexpr int kPerThread = 4;                          // consecutive tokens of a thread in a sweep
+constexpr int kSweep = kSelectThreads * kPerThread;
+constexpr int kBins = 2048;
+
+// Larger weights are larger keys; -0 equals 0, every NaN is the largest.
+__device__ __forceinline__ uint32_t order_key(float w) {
+    if (w != w) return 0xffffffffu;
+    const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.f);  // -0 + 0 = +0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct SelectParams {
+    const float* weights;
+    const int* ctx_lens;
+    int* new_lens;
+    float* new_weights;
+    int* kept;
+    int64_t w_stride_b, w_stride_h;
+    int hkv, length, max_tok, budget, recent;
+};
+
+// Sum over the workgroup of one value per wave; every thread gets it.
+__device__ __forceinline__ int wave_inclusive(int x, int lane) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int y = __shfl_up(x, d, kWave);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const SelectParams a) {
+    __shared__ int hist[kBins];
+    __shared__ int wave_total[kSelectWaves];
+    __shared__ int found_bin, found_above;
+    const int h = blockIdx.x, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+    const int n = max(min(a.ctx_lens[b], a.max_tok), 0);
+    const float* wt = a.weights + b * a.w_stride_b + h * a.w_stride_h;
+    float* new_wt = a.new_weights + ((size_t)b * a.hkv + h) * a.length;
+    int* kept = a.kept + ((size_t)b * a.hkv + h) * a.budget;
+    const int m = min(n, a.budget);
+    if (h == 0 && tid == 0) a.new_lens[b] = m;
+    for (int i = m + tid; i < a.length; i += kSelectThreads) new_wt[i] = 0.f;
+    for (int i = m + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+    if (n <= a.budget) {
+        for (int i = tid; i < n; i += kSelectThreads) {
+            kept[i] = i;
+            new_wt[i] = wt[i];
+        }
+        return;
+    }
+    const int old = n - a.recent, want = a.budget - a.recent;  // 0 <= want < old
+    // The key of the want-th largest of the first `old` tokens: `prefix` holds
+    // its top bits, `above` of the tokens have larger ones.
+    uint32_t prefix = 0xffffffffu;
+    int above = 0;
+    if (want > 0) {
+        uint32_t known = 0;  // mask of the bits found
+        prefix = 0;
+        constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = kShift[pass], bins = 1 << kBits[pass];
+            for (int i = tid; i < bins; i += kSelectThreads) hist[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < old; i += kSelectThreads) {
+                const uint32_t k = order_key(wt[i]);
+                if ((k & known) == prefix) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
+            }
+            __syncthreads();
+            // Bins from the largest down, two of a thread: where the count passes want.
+            const int hi = bins - 1 - 2 * tid;
+            const int c0 = hi >= 0 ? hist[hi] : 0, c1 = hi >= 0 ? hist[hi - 1] : 0;
+            const int inc = wave_inclusive(c0 + c1, lane);
+            if (lane == kWave - 1) wave_total[w] = inc;
+            __syncthreads();
+            int before = above + inc - c0 - c1;
+            for (int v = 0; v < w; ++v) before += wave_total[v];
+            if (before < want && want <= before + c0) {
+                found_bin = hi;
+                found_above = before;
+            } else if (before + c0 < want && want <= before + c0 + c1) {
+                found_bin = hi - 1;
+                found_above = before + c0;
+            }
+            __syncthreads();
+            prefix |= (uint32_t)found_bin << shift;
+            known |= (uint32_t)(bins - 1) << shift;
+            above = found_above;
+        }
+    }
+    const int ties = want - above;  // tokens of that very key that are kept: the first ones (none where want is 0)
+    int gt_before = 0, eq_before = 0;
+    for (int base = 0; base < n; base += kSweep) {
+        const int i0 = base + tid * kPerThread;
+        float x[kPerThread];
+        int gt[kPerThread], eq[kPerThread], packed = 0;
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            const int i = i0 + j;
+            x[j] = i < n ? wt[i] : 0.f;
+            const uint32_t k = order_key(x[j]);
+            gt[j] = i < n && (i >= old || (want > 0 && k > prefix));
+            eq[j] = i < old && want > 0 && k == prefix;
+            packed += gt[j] | eq[j] << 16;
+        }
+        const int inc = wave_inclusive(packed, lane);
+        __syncthreads();  // wave_total of the sweep before has been read
+        if (lane == kWave - 1) wave_total[w] = inc;
+        __syncthreads();
+        int before = inc - packed, total = 0;
+        for (int v = 0; v < kSelectWaves; ++v) {
+            if (v < w) before += wave_total[v];
+            total += wave_total[v];
+        }
+        int g = gt_before + (before & 0xffff), e = eq_before + (before >> 16);
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            if (gt[j] || (eq[j] && e < ties)) {
+                const int to = g + min(e, ties);
+                kept[to] = i0 + j;
+                new_wt[to] = x[j];
+            }
+            g += gt[j];
+            e += eq[j];
+        }
+        gt_before += total & 0xffff;
+        eq_before += total >> 16;
+    }
+}
+
+struct MoveParams {
+    char* rows[4];          // K, V and their scales
+    int row_bytes[4], columns[4];
+    const int *tables, *new_tables, *ctx_lens, *new_lens, *kept;
+    int hkv, bs, bs_shift, max_blocks, new_max_blocks, num_blocks, max_tok, budget;
+    bool in_place;
+};
+
+constexpr int kMoveThreads = 256;
+constexpr int kBatch = 8;       // rows that a lane has in flight
+constexpr int kColumn = 128;    // bytes of a row that a workgroup moves
+
+// U: the bytes that a lane moves at a time.
+template <class U>
+__device__ __forceinline__ void move_rows(const MoveParams& a, char* plane, int row_bytes, int column, int b, int h) {
+    const int width = min(row_bytes - column * kColumn, kColumn) / (int)sizeof(U);  // lanes of a row
+    const int tid = threadIdx.x, per_pass = kMoveThreads / width;
+    const int lane_row = tid / width, offset = column * kColumn + tid % width * (int)sizeof(U);
+    const bool idle = lane_row >= per_pass;
+    const int m = a.new_lens[b];
+    const int* kept = a.kept + ((size_t)b * a.hkv + h) * a.budget;
+    const int* from = a.tables + (size_t)b * a.max_blocks;
+    const int* to = a.new_tables + (size_t)b * a.new_max_blocks;
+    auto locate = [&](const int* table, int i) -> char* {  // null: no such page
+        const int pi = a.bs_shift >= 0 ? i >> a.bs_shift : i / a.bs;
+        const int page = table[pi];
+        if ((unsigned)page >= (unsigned)a.num_blocks) return nullptr;
+        return plane + (((size_t)page * a.hkv + h) * a.bs + (i - pi * a.bs)) * row_bytes + offset;
+    };
+    for (int base = 0; base < m; base += kBatch * per_pass) {
+        U x[kBatch];
+        char* dst[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = base + j * per_pass + lane_row;
+            dst[j] = nullptr;
+            if (idle || i >= m) continue;
+            const int src = kept[i];
+            if (a.in_place && src == i) continue;
+            const char* p = locate(from, src);
+            dst[j] = p ? locate(to, i) : nullptr;
+            if (dst[j]) x[j] = *reinterpret_cast<const U*>(p);
+        }
+        // Every row of the batch has been read before one of them is written.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (dst[j]) *reinterpret_cast<U*>(dst[j]) = x[j];
+    }
+}
+
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const MoveParams a) {
+    const int h = blockIdx.y, b = blockIdx.z;
+    if (a.in_place && min(a.ctx_lens[b], a.max_tok) <= a.budget) return;  // every row stays
+    int plane = 0, column = blockIdx.x;
+    while (column >= a.columns[plane]) column -= a.columns[plane++];
+    const int rb = a.row_bytes[plane];
+    if (rb % 16 == 0) move_rows<u32x4>(a, a.rows[plane], rb, column, b, h);
+    else if (rb % 4 == 0) move_rows<uint32_t>(a, a.rows[plane], rb, column, b, h);
+    else move_rows<uint8_t>(a, a.rows[plane], rb, column, b, h);
+}
+
+}  // namespace
+
+hipError_t evict_launch(const EvictArgs& x) {
+    SelectParams s{};
+    s.weights = x.weights;
+    s.ctx_lens = x.context_lens;
+    s.new_lens = x.new_lens;
+    s.new_weights = x.new_weights;
+    s.kept = x.kept;
+    s.w_stride_b = x.w_stride_b;
+    s.w_stride_h = x.w_stride_h;
+    s.hkv = (int)x.hkv;
+    s.length = (int)x.length;
+    s.max_tok = (int)std::min(x.length, x.max_blocks * x.bs);
+    s.budget = (int)x.budget;
+    s.recent = (int)x.recent;
+    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)x.hkv, (unsigned)x.batch), dim3(kSelectThreads), 0,
+                       (hipStream_t)x.stream, s);
+    MoveParams m{};
+    int columns = 0;
+    for (int i = 0; i < 4 && x.rows[i]; ++i) {
+        m.rows[i] = static_cast<char*>(x.rows[i]);
+        m.row_bytes[i] = (int)x.row_bytes[i];
+        m.columns[i] = (m.row_bytes[i] + kColumn - 1) / kColumn;
+        columns += m.columns[i];
+    }
+    m.tables = x.block_tables;
+    m.new_tables = x.new_block_tables ? x.new_block_tables : x.block_tables;
+    m.in_place = !x.new_block_tables;
+    m.ctx_lens = x.context_lens;
+    m.max_tok = s.max_tok;
+    m.new_lens = x.new_lens;
+    m.kept = x.kept;
+    m.hkv = (int)x.hkv;
+    m.bs = (int)x.bs;
+    m.bs_shift = (x.bs & (x.bs - 1)) == 0 ? __builtin_ctzll((unsigned long long)x.bs) : -1;
+    m.max_blocks = (int)x.max_blocks;
+    m.new_max_blocks = (int)(x.new_block_tables ? x.new_max_blocks : x.max_blocks);
+    m.num_blocks = (int)x.num_blocks;
+    m.budget = (int)x.budget;
+    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)columns, (unsigned)x.hkv, (unsigned)x.batch),
+                       dim3(kMoveThreads), 0, (hipStream_t)x.stream, m);
+    return hipGetLastError();
+}
+
+}  // namespace ak

@@ -14,6 +14,7 @@
 #include <cmath>
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -379,6 +380,266 @@ bool plain_write(py::handle ko, py::handle vo, py::handle kco, py::handle vco, p
     return true;
 }
 
+// ---------------------------------------------------------------------------
+// The smaller cache: 4-bit (MXFP4) caches, attention weights per cached token,
+// eviction.  These are the Python entry points' bodies: every check is made
+// here, in one pass, and raises ValueError; sizes come before devices.
+namespace {
+
+void require(bool fine, const char* message) {
+    if (!fine) throw py::value_error(message);
+}
+
+bool is_half(const torch::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+
+void require_gpu(std::initializer_list<const torch::Tensor*> ts) {
+    const torch::Tensor& first = **ts.begin();
+    for (const torch::Tensor* t : ts)
+        require(t->is_cuda() && t->device() == first.device(), "all tensors must be GPU tensors on the same device");
+}
+
+torch::Tensor aligned(const torch::Tensor& x) {
+    torch::Tensor y = x.contiguous();
+    return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
+}
+
+// Rows that the kernels read as they are: heads contiguous, token stride and start on 16 bytes; else a copy.
+torch::Tensor token_rows(const torch::Tensor& x) {
+    const bool fine = x.stride(2) == 1 && (x.size(1) <= 1 || x.stride(1) == x.size(2)) &&
+                      (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) * x.size(2))) &&
+                      reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    return fine ? x : aligned(x);
+}
+
+int64_t token_stride(const torch::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1) * x.size(2); }
+
+torch::Tensor int_array(const torch::Tensor& x) { return x.to(at::kInt).contiguous(); }
+
+// MXFP4 caches of head size D; the caches' sizes are kc's.
+void check_mx_caches(const torch::Tensor& kc, const torch::Tensor& ks, const torch::Tensor& vc,
+                     const torch::Tensor& vs, int64_t D) {
+    require(D % 32 == 0, "head_dim must be a multiple of 32");
+    for (const auto* t : {&kc, &ks, &vc, &vs})
+        require(t->scalar_type() == at::kByte && t->dim() == 4, "4-bit caches and their scales must be uint8 [num_blocks, "
+                                                                "H_kv, block_size, ...]");
+    require(kc.size(3) == D / 2 && vc.sizes() == kc.sizes(), "k_cache and v_cache must be [num_blocks, H_kv, "
+                                                            "block_size, D / 2] of the same shape");
+    for (const auto* t : {&ks, &vs})
+        require(t->size(0) == kc.size(0) && t->size(1) == kc.size(1) && t->size(2) == kc.size(2) && t->size(3) == D / 32,
+                "k_scales and v_scales must be [num_blocks, H_kv, block_size, D / 32] matching the caches");
+    for (const auto* t : {&kc, &ks, &vc, &vs}) require(t->is_contiguous(), "caches and scales must be contiguous");
+}
+
+// weights: float32 [batch, kv heads, >= length], rows contiguous and apart.
+void check_weights(const torch::Tensor& w, int64_t batch, int64_t hkv, int64_t length) {
+    require(w.scalar_type() == at::kFloat && w.dim() == 3 && w.size(0) == batch && w.size(1) == hkv,
+            "weights must be float32 [B, H_kv, length]");
+    require(w.size(2) >= length, "weights must be at least as long as the longest sequence");
+    require(w.size(2) <= 1 || w.stride(2) == 1, "weights must be contiguous along their last dimension");
+}
+
+torch::Tensor slots_on(const torch::Tensor& slots, const torch::Tensor& rows, int64_t tokens) {
+    require(slots.dim() == 1 && slots.size(0) == tokens, "slot_mapping must be [num_tokens]");
+    require(slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt, "slot_mapping must be int64 or int32");
+    return slots.to(rows.device(), at::kLong).contiguous();  // a host tensor is copied over
+}
+
+}  // namespace
+
+void reshape_and_cache_mxfp4(const torch::Tensor& key, const torch::Tensor& value, const torch::Tensor& kc,
+                             const torch::Tensor& ks, const torch::Tensor& vc, const torch::Tensor& vs,
+                             const torch::Tensor& slot_mapping) {
+    require(key.dim() == 3 && value.sizes() == key.sizes(), "key and value must be [num_tokens, H_kv, D] of the same "
+                                                            "shape");
+    require(is_half(key) && value.scalar_type() == key.scalar_type(), "key and value must both be fp16 or both bf16");
+    const int64_t T = key.size(0), hkv = key.size(1), D = key.size(2);
+    check_mx_caches(kc, ks, vc, vs, D);
+    require(kc.size(1) == hkv, "caches must have the kv heads of key");
+    require(slot_mapping.dim() == 1 && slot_mapping.size(0) == T, "slot_mapping must be [num_tokens]");
+    require_gpu({&key, &value, &kc, &ks, &vc, &vs});
+    const at::hip::HIPGuardMasqueradingAsCUDA guard(key.device());
+    const torch::Tensor slots = slots_on(slot_mapping, key, T), k = token_rows(key), v = token_rows(value);
+    check_rc(ak_reshape_and_cache_mxfp4(k.data_ptr(), v.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(),
+                                        vs.data_ptr(), slots.data_ptr<int64_t>(), T, hkv, D, kc.size(0), kc.size(2),
+                                        token_stride(k), token_stride(v), key.scalar_type() == at::kBFloat16,
+                                        stream_of(key)));
+}
+
+std::pair<torch::Tensor, torch::Tensor> gather_cache_mxfp4(const torch::Tensor& kc, const torch::Tensor& ks,
+                                                           const torch::Tensor& vc, const torch::Tensor& vs,
+                                                           const torch::Tensor& slot_mapping, at::ScalarType dtype) {
+    require(kc.dim() == 4, "k_cache must be [num_blocks, H_kv, block_size, D / 2]");
+    require(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be torch.float16 or torch.bfloat16");
+    const int64_t D = 2 * kc.size(3), T = slot_mapping.dim() == 1 ? slot_mapping.size(0) : -1;
+    check_mx_caches(kc, ks, vc, vs, D);
+    require(T >= 0, "slot_mapping must be [num_tokens]");
+    require_gpu({&kc, &ks, &vc, &vs});
+    const at::hip::HIPGuardMasqueradingAsCUDA guard(kc.device());
+    const torch::Tensor slots = slots_on(slot_mapping, kc, T);
+    auto key = torch::empty({T, kc.size(1), D}, kc.options().dtype(dtype)), value = torch::empty_like(key);
+    check_rc(ak_gather_cache_mxfp4(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), slots.data_ptr<int64_t>(),
+                                   key.data_ptr(), value.data_ptr(), T, kc.size(1), D, kc.size(0), kc.size(2),
+                                   dtype == at::kBFloat16, stream_of(kc)));
+    return {key, value};
+}
+
+// ks, vs: the scales of a 4-bit cache, or null.
+static torch::Tensor decode_mx(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor* ks,
+                               const torch::Tensor& vc, const torch::Tensor* vs, const torch::Tensor& block_tables,
+                               const torch::Tensor& context_lens, int64_t max_ctx, c10::optional<double> scale,
+                               c10::optional<int64_t> partition_size, const torch::Tensor* weights) {
+    require(q.dim() == 3 && is_half(q), "q must be fp16 or bf16 [B, H, D]");
+    const int64_t B = q.size(0), hq = q.size(1), D = q.size(2);
+    require(D == 64 || D == 128, "head_dim must be 64 or 128");
+    if (ks) {
+        check_mx_caches(kc, *ks, vc, *vs, D);
+    } else {
+        require(kc.scalar_type() == q.scalar_type() && vc.scalar_type() == q.scalar_type(),
+                "q and the caches must all be fp16 or all bf16");
+        require(kc.dim() == 4 && vc.sizes() == kc.sizes() && kc.size(3) == D,
+                "caches must be [num_blocks, H_kv, block_size, D] matching q");
+        require(kc.is_contiguous() && vc.is_contiguous(), "caches must be contiguous");
+    }
+    const int64_t hkv = kc.size(1);
+    require(block_tables.dim() == 2 && block_tables.size(0) == B, "block_tables must be [B, max_blocks]");
+    require(context_lens.dim() == 1 && context_lens.size(0) == B, "context_lens must be [B]");
+    require(!c10::isFloatingType(block_tables.scalar_type()) && !c10::isFloatingType(context_lens.scalar_type()),
+            "block_tables and context_lens must be integers");
+    if (weights) check_weights(*weights, B, hkv, max_ctx);
+    require_gpu({&q, &kc, &vc, &block_tables, &context_lens});
+    if (ks) require_gpu({&q, ks, vs});
+    if (weights) require_gpu({&q, weights});
+    const at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    const torch::Tensor q1 = aligned(q), bt = int_array(block_tables), ctx = int_array(context_lens);
+    auto out = torch::empty({B, hq, D}, q.options());
+    const int64_t partition = partition_size.has_value() ? (*partition_size + 255) / 256 * 256
+                                                         : ak_paged_decode_mx_partition(B, hkv, max_ctx);
+    const size_t ws_bytes = ak_paged_decode_mx_workspace_size(B, hq, D, max_ctx, partition, weights != nullptr);
+    torch::Tensor ws, counters;
+    if (ws_bytes > 0) ws = torch::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
+    if (ws_bytes > 0 && !weights) counters = split_counters(q, B * hkv);
+    void* const wsp = ws_bytes > 0 ? ws.data_ptr() : nullptr;
+    float* const wp = weights ? weights->data_ptr<float>() : nullptr;
+    const int64_t wb = weights ? weights->stride(0) : 0, wh = weights ? weights->stride(1) : 0;
+    const int64_t wl = weights ? weights->size(2) : 0;
+    const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)D);
+    const int bf16 = q.scalar_type() == at::kBFloat16;
+    check_rc(ks ? ak_paged_decode_mxfp4(q1.data_ptr(), kc.data_ptr(), ks->data_ptr(), vc.data_ptr(), vs->data_ptr(),
+                                        bt.data_ptr<int32_t>(), ctx.data_ptr<int32_t>(), out.data_ptr(), wp, wb, wh, wl,
+                                        B, hq, hkv, D, kc.size(0), kc.size(2), bt.size(1), max_ctx, s, partition, bf16,
+                                        wsp, ws_bytes, counters.defined() ? counters.data_ptr<int32_t>() : nullptr,
+                                        counters.defined() ? counters.numel() : 0, stream_of(q))
+                : ak_paged_decode_weights(q1.data_ptr(), kc.data_ptr(), vc.data_ptr(), bt.data_ptr<int32_t>(),
+                                          ctx.data_ptr<int32_t>(), out.data_ptr(), wp, wb, wh, wl, B, hq, hkv, D,
+                                          kc.size(0), kc.size(2), bt.size(1), max_ctx, s, partition, bf16, wsp,
+                                          ws_bytes, stream_of(q)));
+    return out;
+}
+
+torch::Tensor paged_decode_mxfp4(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& ks,
+                                 const torch::Tensor& vc, const torch::Tensor& vs, const torch::Tensor& bt,
+                                 const torch::Tensor& ctx, int64_t max_ctx, c10::optional<double> scale,
+                                 c10::optional<int64_t> partition, const c10::optional<torch::Tensor>& weights) {
+    return decode_mx(q, kc, &ks, vc, &vs, bt, ctx, max_ctx, scale, partition, weights.has_value() ? &*weights : nullptr);
+}
+
+torch::Tensor paged_decode_weights(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& vc,
+                                   const torch::Tensor& bt, const torch::Tensor& ctx, int64_t max_ctx,
+                                   const torch::Tensor& weights, c10::optional<double> scale,
+                                   c10::optional<int64_t> partition) {
+    return decode_mx(q, kc, nullptr, vc, nullptr, bt, ctx, max_ctx, scale, partition, &weights);
+}
+
+void prompt_weights(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& cu_seqlens,
+                    int64_t max_seqlen, const torch::Tensor& weights, c10::optional<int64_t> last,
+                    c10::optional<double> scale) {
+    require(q.dim() == 3 && k.dim() == 3 && is_half(q) && k.scalar_type() == q.scalar_type(),
+            "q and k must be [total, H, D] and [total, H_kv, D], both fp16 or both bf16");
+    const int64_t total = q.size(0), hq = q.size(1), D = q.size(2), hkv = k.size(1);
+    require(k.size(0) == total && k.size(2) == D, "k must be [total, H_kv, D] with the total and D of q");
+    require(hkv > 0 && hq > 0 && hq % hkv == 0, "the query heads must be a multiple of the kv heads");
+    require(D == 64 || D == 128, "head_dim must be 64 or 128");
+    require(cu_seqlens.dim() == 1 && cu_seqlens.size(0) >= 1 && !c10::isFloatingType(cu_seqlens.scalar_type()),
+            "cu_seqlens must be integers [B + 1]");
+    require(!last.has_value() || *last >= 1, "last must be at least 1");
+    require(max_seqlen >= 0, "max_seqlen must not be negative");
+    const int64_t B = cu_seqlens.size(0) - 1;
+    check_weights(weights, B, hkv, std::min(max_seqlen, total));
+    if (!cu_seqlens.is_cuda()) {
+        const torch::Tensor c = cu_seqlens.to(at::kLong).contiguous();
+        const int64_t* at = c.data_ptr<int64_t>();
+        require(at[0] >= 0 && at[B] <= total, "cu_seqlens must be non-decreasing offsets into the packed rows");
+        for (int64_t b = 0; b < B; ++b) {
+            require(at[b] <= at[b + 1], "cu_seqlens must be non-decreasing offsets into the packed rows");
+            require(at[b + 1] - at[b] <= max_seqlen, "max_seqlen is shorter than a sequence");
+        }
+    }
+    require_gpu({&q, &k, &weights});
+    const at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    const torch::Tensor cu = cu_seqlens.to(q.device(), at::kInt).contiguous(), q1 = token_rows(q), k1 = token_rows(k);
+    const int64_t count = last.has_value() ? *last : std::max<int64_t>(max_seqlen, 1);
+    const size_t ws_bytes = ak_prompt_weights_workspace_size(B, total, hq, hkv, D, max_seqlen, count);
+    torch::Tensor ws;
+    if (ws_bytes > 0) ws = torch::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
+    check_rc(ak_prompt_weights(q1.data_ptr(), k1.data_ptr(), cu.data_ptr<int32_t>(), weights.data_ptr<float>(),
+                               weights.stride(0), weights.stride(1), weights.size(2), B, total, hq, hkv, D,
+                               token_stride(q1), token_stride(k1), max_seqlen, count,
+                               scale.has_value() ? *scale : 1.0 / std::sqrt((double)D),
+                               q.scalar_type() == at::kBFloat16, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
+                               stream_of(q)));
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> evict_cache(
+    const torch::Tensor& kc, const torch::Tensor& vc, const torch::Tensor& block_tables,
+    const torch::Tensor& context_lens, const torch::Tensor& weights, int64_t budget, int64_t recent,
+    const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs,
+    const c10::optional<torch::Tensor>& new_block_tables) {
+    require(ks.has_value() == vs.has_value(), "k_scales and v_scales come together");
+    if (ks.has_value()) {
+        require(kc.dim() == 4, "caches must be [num_blocks, H_kv, block_size, ...]");
+        check_mx_caches(kc, *ks, vc, *vs, 2 * kc.size(3));
+    } else {
+        require(is_half(kc) && vc.scalar_type() == kc.scalar_type(),
+                "caches must both be fp16 or both bf16 (4-bit ones come with their scales)");
+        require(kc.dim() == 4 && vc.sizes() == kc.sizes(), "caches must be [num_blocks, H_kv, block_size, D]");
+        require(kc.is_contiguous() && vc.is_contiguous(), "caches must be contiguous (they are written in place)");
+    }
+    const int64_t row_bytes = kc.size(3) * kc.element_size();
+    require(row_bytes % 16 == 0 && row_bytes > 0, "a cache row must be a multiple of 16 bytes");
+    require(block_tables.dim() == 2 && context_lens.dim() == 1 && block_tables.size(0) == context_lens.size(0),
+            "block_tables must be [B, max_blocks] and context_lens [B]");
+    require(!c10::isFloatingType(block_tables.scalar_type()) && !c10::isFloatingType(context_lens.scalar_type()),
+            "block_tables and context_lens must be integers");
+    const int64_t B = context_lens.size(0), hkv = kc.size(1);
+    check_weights(weights, B, hkv, 0);
+    require(budget >= 1 && recent >= 0 && recent <= budget, "budget must be at least 1, recent from 0 to budget");
+    const torch::Tensor* nt = new_block_tables.has_value() ? &*new_block_tables : nullptr;
+    if (nt) {
+        require(nt->dim() == 2 && nt->size(0) == B && !c10::isFloatingType(nt->scalar_type()),
+                "new_block_tables must be integers [B, new_max_blocks]");
+        require(nt->size(1) * kc.size(2) >= std::min({budget, weights.size(2), block_tables.size(1) * kc.size(2)}),
+                "new_block_tables must have pages for budget tokens");
+    }
+    require_gpu({&kc, &vc, &block_tables, &context_lens, &weights});
+    if (ks.has_value()) require_gpu({&kc, &*ks, &*vs});
+    if (nt) require_gpu({&kc, nt});
+    const at::hip::HIPGuardMasqueradingAsCUDA guard(kc.device());
+    const torch::Tensor bt = int_array(block_tables), ctx = int_array(context_lens);
+    torch::Tensor new_bt;
+    if (nt) new_bt = int_array(*nt);
+    auto lens = torch::empty({B}, ctx.options());
+    auto new_weights = torch::empty({B, hkv, weights.size(2)}, weights.options());
+    auto kept = torch::empty({B, hkv, budget}, ctx.options());
+    check_rc(ak_evict_cache(kc.data_ptr(), vc.data_ptr(), row_bytes, ks.has_value() ? ks->data_ptr() : nullptr,
+                            vs.has_value() ? vs->data_ptr() : nullptr, ks.has_value() ? ks->size(3) : 0,
+                            bt.data_ptr<int32_t>(), nt ? new_bt.data_ptr<int32_t>() : nullptr, ctx.data_ptr<int32_t>(),
+                            weights.data_ptr<float>(), weights.stride(0), weights.stride(1), weights.size(2),
+                            lens.data_ptr<int32_t>(), new_weights.data_ptr<float>(), kept.data_ptr<int32_t>(), B, hkv,
+                            kc.size(0), kc.size(2), bt.size(1), nt ? new_bt.size(1) : 0, budget, recent,
+                            stream_of(kc)));
+    return {lens, new_weights, kept};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "gfx950 attention kernels: MFMA flash prefill, paged split-K decode";
     m.def("naive_attention", &naive_attention, "prefill attention (served by the MFMA flash kernel)");
@@ -395,4 +656,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("plain_write", &plain_write, "reshape_and_cache on plain arguments, else False");
     m.def("flash_gqa", &flash_gqa, "dense prefill with grouped-query attention");
     m.def("flash_varlen", &flash_varlen, "prefill over packed variable-length sequences");
+    m.def("reshape_and_cache_mxfp4", &reshape_and_cache_mxfp4, "write new tokens' K/V rows into 4-bit paged caches");
+    m.def("gather_cache_mxfp4", &gather_cache_mxfp4, "the values of slots of 4-bit paged caches");
+    m.def("paged_decode_mxfp4", &paged_decode_mxfp4, "decode attention over 4-bit paged caches");
+    m.def("paged_decode_weights", &paged_decode_weights, "decode attention that sums its weights per cached token");
+    m.def("prompt_weights", &prompt_weights, "attention weights of a prompt's queries, summed per token");
+    m.def("evict_cache", &evict_cache, "keep the last and the heaviest tokens of paged caches");
 }

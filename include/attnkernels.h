@@ -213,6 +213,113 @@ int ak_reshape_and_cache(const void *key, const void *value, void *k_cache, void
                          int64_t head_dim, int64_t num_blocks, int64_t block_size,
                          int64_t key_stride, int64_t value_stride, void *stream);
 
+/* ---- A smaller KV cache: four bits a value, fewer tokens (no counterpart in
+ * the reference, whose cache is fp16 and only read).  Elements of q, key, value,
+ * out and full-precision caches are fp16, or bf16 where `bf16` is not 0.
+ *
+ * MXFP4 caches: 32 channels of one token and head share a scale byte s for
+ * 2^(s - 127), 255: the group reads NaN; a value is a 4-bit code, a sign (bit 3)
+ * and one of 0, .5, 1, 1.5, 2, 3, 4, 6.  Codes: [num_blocks, num_kv_heads,
+ * block_size, head_dim / 2] bytes, the even channel in the low half; scales:
+ * [num_blocks, num_kv_heads, block_size, head_dim / 32] bytes.
+ *
+ * Attention weights: float [batch, num_kv_heads, length], a kv head's row
+ * weights_stride_h and a sequence's weights_stride_b elements after the one
+ * before (rows must not overlap); the sum of the softmax weights that a cached
+ * token got, over the query heads of its kv head and over calls. */
+
+/* ak_reshape_and_cache into MXFP4 caches.  The scale's exponent is that of the
+ * group's largest magnitude, rounded to two significant bits, less 2, and at
+ * least -126; codes are rounded to nearest even; a group that holds an infinity
+ * or a NaN gets the scale 255.  head_dim a multiple of 32 up to 512. */
+int ak_reshape_and_cache_mxfp4(const void *key, const void *value, void *k_cache, void *k_scales,
+                               void *v_cache, void *v_scales, const int64_t *slot_mapping,
+                               int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t num_blocks, int64_t block_size, int64_t key_stride,
+                               int64_t value_stride, int bf16, void *stream);
+
+/* Its inverse: the values of the slots as key, value [num_tokens, num_kv_heads,
+ * head_dim], rounded to nearest even where the type does not hold them; zeros
+ * for slots that ak_reshape_and_cache_mxfp4 would skip. */
+int ak_gather_cache_mxfp4(const void *k_cache, const void *k_scales, const void *v_cache,
+                          const void *v_scales, const int64_t *slot_mapping, void *key, void *value,
+                          int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                          int64_t num_blocks, int64_t block_size, int bf16, void *stream);
+
+/* Tokens per split that suit these sizes (a multiple of 256), and the workspace
+ * of the two calls below: with_weights != 0 where weights are given. 0 bytes:
+ * none is needed; 0 too for invalid sizes. */
+int64_t ak_paged_decode_mx_partition(int64_t batch, int64_t num_kv_heads, int64_t max_context_len);
+size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64_t head_dim,
+                                         int64_t max_context_len, int64_t partition, int with_weights);
+
+/* Paged decode over MXFP4 caches, num_heads / num_kv_heads from 1 to 16, and,
+ * where weights is not NULL, weights[b, kv head, t] += sum over the kv head's
+ * query heads of token t's softmax weight.  Tokens at or past
+ * max_context_len are ignored; weights_length >= max_context_len.  Arguments
+ * otherwise as in ak_paged_decode_fused (counters may be NULL; they are not used
+ * with weights). */
+int ak_paged_decode_mxfp4(const void *q, const void *k_cache, const void *k_scales, const void *v_cache,
+                          const void *v_scales, const int32_t *block_tables, const int32_t *context_lens,
+                          void *out, float *weights, int64_t weights_stride_b, int64_t weights_stride_h,
+                          int64_t weights_length, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                          int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                          int64_t max_blocks_per_seq, int64_t max_context_len, double scale,
+                          int64_t partition, int bf16, void *workspace, size_t workspace_bytes,
+                          int32_t *counters, int64_t counters_len, void *stream);
+
+/* The same over fp16 or bf16 caches [num_blocks, num_kv_heads, block_size,
+ * head_dim]; weights is required (without: ak_paged_decode). */
+int ak_paged_decode_weights(const void *q, const void *k_cache, const void *v_cache,
+                            const int32_t *block_tables, const int32_t *context_lens, void *out,
+                            float *weights, int64_t weights_stride_b, int64_t weights_stride_h,
+                            int64_t weights_length, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                            int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                            int64_t max_blocks_per_seq, int64_t max_context_len, double scale,
+                            int64_t partition, int bf16, void *workspace, size_t workspace_bytes,
+                            void *stream);
+
+/* What causal prefill of packed sequences gave each of their tokens: weights[b,
+ * kv, j] = the sum over the kv head's query heads and over the sequence's last
+ * `last` queries i >= j of softmax_j(scale q_i.k_j, j <= i), 0 from the sequence's
+ * length on.  q [total_rows, num_heads, head_dim] and k [total_rows, num_kv_heads,
+ * head_dim] with token strides in elements (multiples of 8; heads contiguous);
+ * cu_seqlens and max_seqlen as in ak_prefill_varlen, max_seqlen <= weights_length. */
+size_t ak_prompt_weights_workspace_size(int64_t batch, int64_t total_rows, int64_t num_heads,
+                                        int64_t num_kv_heads, int64_t head_dim, int64_t max_seqlen,
+                                        int64_t last);
+int ak_prompt_weights(const void *q, const void *k, const int32_t *cu_seqlens, float *weights,
+                      int64_t weights_stride_b, int64_t weights_stride_h, int64_t weights_length,
+                      int64_t batch, int64_t total_rows, int64_t num_heads, int64_t num_kv_heads,
+                      int64_t head_dim, int64_t q_stride, int64_t k_stride, int64_t max_seqlen,
+                      int64_t last, double scale, int bf16, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+/* Eviction: a sequence longer than `budget` tokens keeps, for each kv head, its
+ * last `recent` tokens and of the others the budget - recent of the largest
+ * weight (NaN counts as the largest; of equal ones the first), in their order.
+ *   new_lens     int32 [batch]: min(context length, budget)
+ *   new_weights  float [batch, num_kv_heads, weights_length], the kept tokens'
+ *                weights and zeros (not the memory of weights)
+ *   kept         int32 [batch, num_kv_heads, budget]: position i's token was at
+ *                kept[i]; -1 from new_lens on
+ *   k_cache, v_cache  rows of row_bytes bytes (a multiple of 16 up to 1024);
+ *                k_scales, v_scales rows of scale_bytes bytes, or NULL and 0
+ *   new_block_tables  NULL: row i of a sequence's pages becomes what row kept[i]
+ *                was, rows from new_lens on stay; then no page may be in two
+ *                sequences of which one is cut.  Else int32 [batch,
+ *                new_max_blocks]: all kept rows are written to these pages, none
+ *                of which may be in block_tables or there twice.
+ * Tokens past weights_length or the block table's row are ignored; rows on page
+ * ids outside [0, num_blocks) are neither read nor written. */
+int ak_evict_cache(void *k_cache, void *v_cache, int64_t row_bytes, void *k_scales, void *v_scales,
+                   int64_t scale_bytes, const int32_t *block_tables, const int32_t *new_block_tables,
+                   const int32_t *context_lens, const float *weights, int64_t weights_stride_b,
+                   int64_t weights_stride_h, int64_t weights_length, int32_t *new_lens,
+                   float *new_weights, int32_t *kept, int64_t batch, int64_t num_kv_heads,
+                   int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                   int64_t new_max_blocks, int64_t budget, int64_t recent, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
