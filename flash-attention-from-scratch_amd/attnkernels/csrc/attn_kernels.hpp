@@ -149,6 +149,7 @@ struct PromptWeightsArgs {
     void* stream;
 };
 hipError_t prompt_weights_launch(const PromptWeightsArgs& a);
+bool prompt_weights_fits(const PromptWeightsArgs& a);  // whether its launches hold that many workgroups
 size_t prompt_weights_workspace(int64_t batch, int64_t total, int64_t hq, int64_t hkv, int64_t max_seqlen,
                                 int64_t last);
 

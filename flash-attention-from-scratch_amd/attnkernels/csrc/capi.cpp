@@ -635,8 +635,9 @@ int ak_prompt_weights(const void* q, const void* k, const int32_t* cu_seqlens, f
                                              "aligned");
     if (q_stride % 8 || k_stride % 8 || q_stride < num_heads * head_dim || k_stride < num_kv_heads * head_dim)
         return fail(AK_ERR_INVALID_ARGUMENT, "prompt_weights: token strides must be multiples of 8 and hold all heads");
-    if (total_rows > INT_MAX / 2 || weights_length > INT_MAX / 2 || batch > 65535 || num_heads > 65535 ||
-        num_heads * ((std::min(last, longest) + 1023) / 1024) > 65535)
+    // Offsets inside a tile of 64 rows are 32 bits wide.
+    if (q_stride > 1 << 24 || k_stride > 1 << 24 || total_rows > INT_MAX / 2 || weights_length > INT_MAX / 2 ||
+        batch > 65535 || num_heads > 65535)
         return fail(AK_ERR_INVALID_ARGUMENT, "prompt_weights: size out of range");
     if (const int rc = weights_rows(who, batch, num_kv_heads, weights_stride_b, weights_stride_h, weights_length))
         return rc;
@@ -668,6 +669,7 @@ int ak_prompt_weights(const void* q, const void* k, const int32_t* cu_seqlens, f
     a.bf16 = bf16 != 0;
     a.sl2 = (float)(scale * kLog2e);
     a.stream = stream;
+    if (!ak::prompt_weights_fits(a)) return fail(AK_ERR_INVALID_ARGUMENT, "prompt_weights: size out of range");
     return hip_status(ak::prompt_weights_launch(a), who);
 }
 

@@ -403,10 +403,12 @@ torch::Tensor aligned(const torch::Tensor& x) {
     return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
 }
 
-// Rows that the kernels read as they are: heads contiguous, token stride and start on 16 bytes; else a copy.
+// Rows that the kernels read as they are: heads contiguous, token stride (up to 2^24 elements) and start on 16 bytes;
+// else a copy.
 torch::Tensor token_rows(const torch::Tensor& x) {
     const bool fine = x.stride(2) == 1 && (x.size(1) <= 1 || x.stride(1) == x.size(2)) &&
-                      (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) * x.size(2))) &&
+                      (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) * x.size(2) &&
+                                           x.stride(0) <= 1 << 24)) &&
                       reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
     return fine ? x : aligned(x);
 }

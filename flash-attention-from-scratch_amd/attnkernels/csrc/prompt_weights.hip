@@ -18,9 +18,10 @@
 //   * prompt_join_kernel adds in a fixed order.
 // Bound by the matrix cores and the exponentials: 2 * 2 D FLOP and two
 // exponentials a score.  The maximum subtracted in the first pass is the one of
-// the first tile unless a sum passes 2^80: sums are in fp32, whose exponent has
+// the first tile unless a sum passes 2^100: sums are in fp32, whose exponent has
 // room for the rest.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_kernels.hpp"
 #include "mxfp4.hpp"
@@ -33,6 +34,8 @@ constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kCols = 64;             // columns that a wave holds
 constexpr int kHeld = kWaves * kCols; // of a workgroup
 constexpr int kTile = 64;             // rows of a streamed tile
+constexpr int kRing = 3;              // tiles in LDS: one in use, two on their way
+constexpr int kRows = 512;            // queries whose maxima and sums a workgroup of the second pass has in LDS
 constexpr float kLowest = -3.402823466e38f;
 
 struct Params {
@@ -43,7 +46,8 @@ struct Params {
     float* partial;        // [items, hkv, total]
     int64_t q_stride, k_stride, w_stride_b, w_stride_h;
     int total, hkv, group, max_seqlen, last, length;
-    int key_range, key_splits, row_range, ranges;
+    int key_range, key_splits, heads, items_h, row_range, ranges;
+    int pairs, key_tiles;  // (sequence, kv head) pairs, the fastest part of a workgroup's number: one's keys meet in one L2
     float sl2;
 };
 
@@ -65,34 +69,56 @@ struct Rows {
     int64_t stride;
 };
 
+// 16-byte units of a row, and of a tile that one thread moves.
 template <int D>
-struct Stream {
-    static constexpr int UNITS = D / 8;                       // 16-byte units of a row
-    static constexpr int PER = kTile * UNITS / kThreads;      // units of a thread
-    u32x4 x[PER];
+constexpr int kUnits = D / 8;
+template <int D>
+constexpr int kPer = kTile * kUnits<D> / kThreads;
 
-    // Where unit u of tile row r stands in LDS: 16 consecutive rows' same units
-    // are on 16 different places of the 256 bytes that one read group covers.
-    static __device__ __forceinline__ int place(int r, int u) {
-        return D == 128 ? r * 16 + (u ^ (r & 15)) : r * 8 + (u ^ (r >> 1 & 7));
-    }
-    // Rows i0 + r, those past `end` as row end - 1.
-    __device__ __forceinline__ void load(const Rows& rows, int i0, int end, int tid) {
+// Where unit u of tile row r stands in LDS: 16 consecutive rows' same units
+// are on 16 different places of the 256 bytes that one read group covers.
+template <int D>
+__device__ __forceinline__ int place(int r, int u) {
+    return D == 128 ? r * 16 + (u ^ (r & 15)) : r * 8 + (u ^ (r >> 1 & 7));
+}
+
+// Starts rows i0 .. of `rows` (those past `end` as row end - 1) on their way
+// into a tile, straight from memory: a wave's 64 lanes fill 1 KB of it, each
+// lane with the unit that belongs to its place.  A tile of whole rows has a
+// scalar base and the same 32-bit offsets every time.  In asm so that the
+// compiler's waits for LDS reads do not wait for these too; tile_ready waits.
+// s_nop 4: the wait states for a base that a vector instruction has just
+// written (a spilled scalar's v_readlane), which the compiler cannot see in asm;
+// they cover the write of M0 too.
+template <int D>
+__device__ __forceinline__ void load_tile(const Rows& rows, int i0, int end, u32x4* tile, int w, int lane) {
+    const uint16_t* base = rows.p + (int64_t)i0 * rows.stride;
+    const bool whole = i0 + kTile <= end;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int id = tid + j * kThreads, r = id / UNITS, u = id % UNITS;
-            const int i = min(i0 + r, end - 1);
-            x[j] = *reinterpret_cast<const u32x4*>(rows.p + i * rows.stride + u * 8);
+    for (int j = 0; j < kPer<D>; ++j) {
+        const int at = (j * kWaves + w) * kWave + lane, r = at / kUnits<D>, p = at % kUnits<D>;
+        const int u = D == 128 ? p ^ (r & 15) : p ^ (r >> 1 & 7);
+        typedef __attribute__((address_space(3))) void lds_void;
+        const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(lds_void*)(tile + (j * kWaves + w) * kWave));
+        if (whole) {
+            const uint32_t off = ((uint32_t)r * (uint32_t)rows.stride + u * 8) * 2;
+            asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(l) : "memory");
+        } else {
+            const uint16_t* g = rows.p + (int64_t)min(i0 + r, end - 1) * rows.stride + u * 8;
+            asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(l) : "memory");
         }
     }
-    __device__ __forceinline__ void store(u32x4* tile, int tid) const {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int id = tid + j * kThreads;
-            tile[place(id / UNITS, id % UNITS)] = x[j];
-        }
-    }
-};
+}
+
+// Waits until the oldest tile is there, `later` tiles (at most kRing - 2) having
+// been started after it, and until every wave is done with the one before.
+template <int D>
+__device__ __forceinline__ void tile_ready(int later) {
+    static_assert(kRing == 3, "one tile may be on its way behind the one that is waited for");
+    if (later > 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPer<D>) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
 
 // Scores (unscaled) of the tile's rows 32 blk .. 32 blk + 31 against the held columns.
 template <int D, class T>
@@ -104,7 +130,7 @@ __device__ __forceinline__ void product(const u32x4* tile, int blk, const u32x4 
         for (int i = 0; i < 16; ++i) s[c][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-        const u32x4 row = tile[Stream<D>::place(32 * blk + (lane & 31), 2 * k + (lane >> 5))];
+        const u32x4 row = tile[place<D>(32 * blk + (lane & 31), 2 * k + (lane >> 5))];
         s[0] = Half<T>::mfma32(row, held[0][k], s[0]);
         s[1] = Half<T>::mfma32(row, held[1][k], s[1]);
     }
@@ -121,92 +147,95 @@ __device__ __forceinline__ void hold(const Rows& rows, int i0, int end, int lane
     }
 }
 
-// Tiles of rows [begin, end) through LDS: use(tile, first row, rows' end) once for each, by every wave.
-template <int D, class Use, class Stage>
-__device__ __forceinline__ void stream(const Rows& rows, int begin, int end, u32x4 (&tiles)[2][kTile * D / 8], int tid,
-                                       Stage stage, Use use) {
-    Stream<D> next;
-    next.load(rows, begin, end, tid);
-    next.store(tiles[0], tid);
-    stage(begin, 0);
-    if (begin + kTile < end) next.load(rows, begin + kTile, end, tid);
-    __syncthreads();
-    int cur = 0;
-    for (int i = begin; i < end; i += kTile, cur ^= 1) {
-        if (i + kTile < end) {
-            next.store(tiles[cur ^ 1], tid);
-            stage(i + kTile, cur ^ 1);
-            if (i + 2 * kTile < end) next.load(rows, i + 2 * kTile, end, tid);
-        }
-        use(tiles[cur], i, cur);
-        __syncthreads();
-    }
-}
-
 // The row of register r of a 32 x 32 product in this lane.
 __device__ __forceinline__ int row_of(int r, int lane) { return 8 * (r / 4) + 4 * (lane >> 5) + r % 4; }
 
 template <int D, class T>
-__global__ void __launch_bounds__(kThreads) prompt_stats_kernel(const Params a) {
-    __shared__ u32x4 tiles[2][kTile * D / 8];
-    const int kvh = blockIdx.y, b = blockIdx.z;
+__global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params a) {
+    __shared__ u32x4 tiles[kRing][kTile * kUnits<D>];
+    const int pair = blockIdx.x % a.pairs, kvh = pair % a.hkv, b = pair / a.hkv;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int G = a.group;
     const Sequence sq = sequence(a, b);
     const int R = sq.n - sq.first;
     const int chunks = (R + kCols - 1) / kCols * G;
     // The longest streams first: the last queries have the lowest workgroup numbers.
-    const int groups = (chunks + kWaves - 1) / kWaves;
-    const int part = blockIdx.x % a.key_splits, group = groups - 1 - (int)blockIdx.x / a.key_splits;
+    const int groups = (chunks + kWaves - 1) / kWaves, index = blockIdx.x / a.pairs;
+    const int part = index % a.key_splits, group = groups - 1 - index / a.key_splits;
     if (group < 0) return;
     const int chunk = min(group * kWaves + w, chunks - 1);
     const int h = kvh * G + chunk % G, q0 = sq.first + chunk / G * kCols;  // position of the wave's first query
     const bool spare = group * kWaves + w >= chunks;
     const int last_chunk = min(group * kWaves + kWaves, chunks) - 1;
-    const int k_begin = part * a.key_range;
-    const int k_end = min(min(sq.first + (last_chunk / G + 1) * kCols, sq.n), k_begin + a.key_range);
+    const int begin = part * a.key_range;
+    const int end = min(min(sq.first + (last_chunk / G + 1) * kCols, sq.n), begin + a.key_range);
+    const int count = begin < end ? (end - begin + kTile - 1) / kTile : 0;
+    const Rows keys{a.k + (int64_t)sq.start * a.k_stride + kvh * D, a.k_stride};
+    const Rows queries{a.q + (int64_t)sq.start * a.q_stride + h * D, a.q_stride};
+    for (int t = 0; t < kRing - 1 && t < count; ++t) load_tile<D>(keys, begin + t * kTile, end, tiles[t], w, lane);
+    u32x4 held[2][D / 16];
+    hold<D>(queries, q0, sq.n, lane, held);
+
     float m[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f};
-    if (k_begin < k_end) {
-        const Rows keys{a.k + (int64_t)sq.start * a.k_stride + kvh * D, a.k_stride};
-        const Rows queries{a.q + (int64_t)sq.start * a.q_stride + h * D, a.q_stride};
-        u32x4 held[2][D / 16];
-        hold<D>(queries, q0, sq.n, lane, held);
-        stream<D>(keys, k_begin, k_end, tiles, tid, [](int, int) {}, [&](const u32x4* tile, int k0, int) {
-            if (spare || k0 > q0 + kCols - 1) return;
+    // Adds a tile's exponentials to l.
+    auto add = [&](const u32x4* tile, int k0, auto masked) {
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk) {
-                const int kb = k0 + 32 * blk;
-                f32x16 s[2];
-                product<D, T>(tile, blk, held, lane, s);
+        for (int blk = 0; blk < 2; ++blk) {
+            const int kb = k0 + 32 * blk;
+            f32x16 s[2];
+            product<D, T>(tile, blk, held, lane, s);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int qc = q0 + 32 * c;
+            for (int c = 0; c < 2; ++c) {
+                int limit = min(q0 + 32 * c + (lane & 31), end - 1) - kb;  // the last key that counts
+                if (decltype(masked)::value) asm volatile("" : "+v"(limit));  // not compared ahead of the branch
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[c][r] *= a.sl2;
-                    if (kb + 31 > qc || kb + 32 > k_end) {  // keys after a query, or past the range
-                        const int limit = min(qc + (lane & 31), k_end - 1) - kb;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[c][r] = row_of(r, lane) > limit ? -INFINITY : s[c][r];
-                    }
-                    auto sum = [&]() {
-                        float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) t[r % 4] += exp2_fast(s[c][r] - m[c]);
-                        return (t[0] + t[1]) + (t[2] + t[3]);
-                    };
-                    float add = sum();
-                    if (__builtin_amdgcn_ballot_w64(!(add <= 0x1p80f))) {
-                        float mx = m[c];
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[c][r]);
-                        l[c] *= exp2_fast(m[c] - mx);
-                        m[c] = mx;
-                        add = sum();
-                    }
-                    l[c] += add;
+                for (int r = 0; r < 16; ++r) {
+                    float x = s[c][r] * a.sl2 - m[c];
+                    if (decltype(masked)::value) x = row_of(r, lane) > limit ? -INFINITY : x;
+                    t[r % 4] += exp2_fast(x);
                 }
+                l[c] += (t[0] + t[1]) + (t[2] + t[3]);
             }
-        });
+        }
+    };
+    auto raise = [&](const u32x4* tile, int k0) {  // m to the tile's maximum
+        float mx[2] = {m[0], m[1]};
+#pragma unroll 1
+        for (int blk = 0; blk < 2; ++blk) {
+            const int kb = k0 + 32 * blk;
+            f32x16 s[2];
+            product<D, T>(tile, blk, held, lane, s);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int limit = min(q0 + 32 * c + (lane & 31), end - 1) - kb;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx[c] = fmaxf(mx[c], row_of(r, lane) > limit ? kLowest : s[c][r] * a.sl2);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            l[c] *= exp2_fast(m[c] - mx[c]);
+            m[c] = mx[c];
+        }
+    };
+    for (int t = 0, cur = 0; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
+        const int k0 = begin + t * kTile;
+        tile_ready<D>(count - 1 - t);
+        if (t + kRing - 1 < count)
+            load_tile<D>(keys, k0 + (kRing - 1) * kTile, end, tiles[cur == 0 ? kRing - 1 : cur - 1], w, lane);
+        if (spare || k0 > q0 + kCols - 1) continue;
+        const u32x4* tile = tiles[cur];
+        const float l0 = l[0], l1 = l[1];
+        const bool masked = k0 + kTile - 1 > q0 || k0 + kTile > end;
+        // The maximum subtracted stays unless the sums pass 2^100; then the tile is done again.
+        for (bool again = false;; again = true) {
+            masked ? add(tile, k0, std::true_type{}) : add(tile, k0, std::false_type{});
+            if (again || !__builtin_amdgcn_ballot_w64(!(l[0] <= 0x1p100f) || !(l[1] <= 0x1p100f))) break;
+            l[0] = l0;
+            l[1] = l1;
+            raise(tile, k0);
+        }
     }
     if (spare) return;
     // A column's rows are in two lanes.
@@ -231,45 +260,59 @@ __device__ __forceinline__ bool reaches(const Params& a, const Sequence& sq, int
 }
 
 template <int D, class T>
-__global__ void __launch_bounds__(kThreads) prompt_sums_kernel(const Params a) {
-    __shared__ u32x4 tiles[2][kTile * D / 8];
-    __shared__ f32x4 row_m[2][kTile / 4], row_w[2][kTile / 4];
-    const int kt = blockIdx.x, kvh = blockIdx.y % a.hkv, b = blockIdx.z;
-    const int item = blockIdx.y / a.hkv, head = item / a.ranges, j = item % a.ranges;
+__global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a) {
+    __shared__ u32x4 tiles[kRing][kTile * kUnits<D>];
+    __shared__ f32x4 row_m[kRows / 4], row_w[kRows / 4];
+    // The last ranges, which all keys stream, first.
+    const int pair = blockIdx.x % a.pairs, kvh = pair % a.hkv, b = pair / a.hkv;
+    int index = blockIdx.x / a.pairs;
+    const int part = index % a.items_h, head0 = part * a.heads;
+    index /= a.items_h;
+    const int kt = index % a.key_tiles, j = a.ranges - 1 - index / a.key_tiles, item = part * a.ranges + j;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const Sequence sq = sequence(a, b);
     if (kt * kHeld >= sq.n || !reaches(a, sq, j, kt)) return;
-    const int h = kvh * a.group + head;
+    const int heads = min(a.heads, a.group - head0), h0 = kvh * a.group + head0;
     const int k0 = kt * kHeld + w * kCols;
     const int lo = sq.first + j * a.row_range, end = min(sq.n, lo + a.row_range);
     const int begin = lo + max(kt * kHeld - lo, 0) / kTile * kTile;
+    const int per_head = (end - begin + kTile - 1) / kTile, count = per_head * heads;
     const Rows keys{a.k + (int64_t)sq.start * a.k_stride + kvh * D, a.k_stride};
-    const Rows queries{a.q + (int64_t)sq.start * a.q_stride + h * D, a.q_stride};
+    Rows queries{a.q + (int64_t)sq.start * a.q_stride + (int64_t)h0 * D, a.q_stride};
+    // Tiles go through the range's queries head by head; the loads run kRing - 1 tiles ahead.
+    int ahead = 0;
+    auto load_next = [&](int buf) {
+        load_tile<D>(queries, begin + ahead * kTile, end, tiles[buf], w, lane);
+        if (++ahead == per_head) {
+            ahead = 0;
+            queries.p += D;
+        }
+    };
+    for (int t = 0; t < kRing - 1 && t < count; ++t) load_next(t);
     u32x4 held[2][D / 16];
     hold<D>(keys, k0, sq.n, lane, held);
-    float sum[2] = {0.f, 0.f};
-    auto stage = [&](int i0, int buf) {  // the tile's rows: maximum and 1 / sum
-        if (tid >= kTile) return;
-        const int i = i0 + tid;
-        float m = INFINITY, wgt = 0.f;  // past the end: weighs nothing
-        if (i < end) {
+    // Every row's maximum and 1 / sum over the key splits; rows past the end weigh nothing.
+    for (int i = tid; i < count * kTile; i += kThreads) {
+        const int head = i / (per_head * kTile), pos = begin + i % (per_head * kTile);
+        float m = INFINITY, wgt = 0.f;
+        if (pos < end) {
             const size_t step = (size_t)a.hkv * a.group * a.total;
-            const size_t at = (size_t)h * a.total + sq.start + i;
-            float M = kLowest, L = 0.f;
+            const size_t at = (size_t)(h0 + head) * a.total + sq.start + pos;
+            float L = 0.f;
+            m = kLowest;
             for (int p = 0; p < a.key_splits; ++p) {
-                const float lp = a.l[at + p * step], mp = lp == 0.f ? kLowest : a.m[at + p * step];
-                const float mx = fmaxf(M, mp);
-                L = L * exp2_fast(M - mx) + lp * exp2_fast(mp - mx);
-                M = mx;
+                const float lp = a.l[at + p * step], mp = a.m[at + p * step];
+                const float mx = lp == 0.f ? m : fmaxf(m, mp);
+                L = L * exp2_fast(m - mx) + (lp == 0.f ? 0.f : lp * exp2_fast(mp - mx));
+                m = mx;
             }
-            m = M;
             wgt = L == 0.f ? 0.f : 1.f / L;  // every score -inf: nothing
         }
-        reinterpret_cast<float*>(row_m[buf])[tid] = m;
-        reinterpret_cast<float*>(row_w[buf])[tid] = wgt;
-    };
-    stream<D>(queries, begin, end, tiles, tid, stage, [&](const u32x4* tile, int i0, int buf) {
-        if (i0 + kTile <= k0) return;  // every query before the wave's keys
+        reinterpret_cast<float*>(row_m)[i] = m;
+        reinterpret_cast<float*>(row_w)[i] = wgt;
+    }
+    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    auto add = [&](const u32x4* tile, int t, int i0, auto masked) {
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
             const int ib = i0 + 32 * blk;
@@ -278,26 +321,35 @@ __global__ void __launch_bounds__(kThreads) prompt_sums_kernel(const Params a) {
             f32x4 m[4], wgt[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                m[r] = row_m[buf][8 * blk + 2 * r + (lane >> 5)];
-                wgt[r] = row_w[buf][8 * blk + 2 * r + (lane >> 5)];
+                m[r] = row_m[16 * t + 8 * blk + 2 * r + (lane >> 5)];
+                wgt[r] = row_w[16 * t + 8 * blk + 2 * r + (lane >> 5)];
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int kc = k0 + 32 * c;
-                const bool cut = ib < kc + 31;  // queries before a key
-                const int limit = kc + (lane & 31) - ib;
+                int limit = k0 + 32 * c + (lane & 31) - ib;  // the first query that sees the key
+                if (decltype(masked)::value) asm volatile("" : "+v"(limit));  // not compared ahead of the branch
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     float x = s[c][r] * a.sl2 - m[r / 4][r % 4];
-                    if (cut) x = row_of(r, lane) < limit ? -INFINITY : x;
-                    sum[c] = fmaf(exp2_fast(x), wgt[r / 4][r % 4], sum[c]);
+                    if (decltype(masked)::value) x = row_of(r, lane) < limit ? -INFINITY : x;
+                    sum[c][r % 2] = fmaf(exp2_fast(x), wgt[r / 4][r % 4], sum[c][r % 2]);
                 }
             }
         }
-    });
+    };
+    for (int t = 0, cur = 0, i0 = begin; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
+        tile_ready<D>(count - 1 - t);
+        if (t + kRing - 1 < count) load_next(cur == 0 ? kRing - 1 : cur - 1);
+        if (i0 + kTile > k0) {  // else every query is before the wave's keys
+            if (i0 < k0 + kCols - 1) add(tiles[cur], t, i0, std::true_type{});
+            else add(tiles[cur], t, i0, std::false_type{});
+        }
+        i0 += kTile;
+        if (i0 >= end) i0 = begin;
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const float both = sum[c] + __shfl_xor(sum[c], 32, kWave);
+        const float one = sum[c][0] + sum[c][1], both = one + __shfl_xor(one, 32, kWave);
         const int i = k0 + 32 * c + (lane & 31);
         if (lane < 32 && i < sq.n) a.partial[((size_t)item * a.hkv + kvh) * a.total + sq.start + i] = both;
     }
@@ -309,30 +361,49 @@ __global__ void __launch_bounds__(kThreads) prompt_join_kernel(const Params a) {
     const Sequence sq = sequence(a, b);
     float sum = 0.f;
     if (i < sq.n)
-        for (int head = 0; head < a.group; ++head)
+        for (int item = 0; item < a.items_h; ++item)
             for (int j = 0; j < a.ranges; ++j)
                 if (reaches(a, sq, j, i / kHeld))
-                    sum += a.partial[((size_t)(head * a.ranges + j) * a.hkv + kvh) * a.total + sq.start + i];
+                    sum += a.partial[((size_t)(item * a.ranges + j) * a.hkv + kvh) * a.total + sq.start + i];
     a.weights[b * a.w_stride_b + kvh * a.w_stride_h + i] = sum;
 }
 
-// How the work is cut.  Key splits of the first pass: enough workgroups for two
-// a CU where few queries count.  Ranges of the second: of at least 1024 queries.
+// How the work is cut.  First pass: keys are split where few queries count, for
+// two workgroups a CU.  Second pass: an item is a range of at most kRows queries
+// of one head, or several heads' queries where a head has few of them and enough
+// workgroups are left.
 struct Plan {
-    int64_t rows, key_range, key_splits, row_range, ranges;
+    int64_t key_range, key_splits, heads, items_h, row_range, ranges;
 };
 
 Plan make_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t max_seqlen, int64_t last) {
     Plan p;
-    p.rows = std::min(last, max_seqlen);
-    const int64_t groups = ((p.rows + kCols - 1) / kCols * (hq / hkv) + kWaves - 1) / kWaves;
+    const int64_t rows = std::min(last, max_seqlen), group = hq / hkv, per_group = batch * hkv;
+    const int64_t groups = ((rows + kCols - 1) / kCols * group + kWaves - 1) / kWaves;
     const int64_t most = (max_seqlen + 255) / 256;  // ranges of at least 256 keys
-    const int64_t want = std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(1, groups * hkv * batch)));
+    const int64_t want = std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(1, groups * per_group)));
     p.key_range = ((max_seqlen + want - 1) / want + kTile - 1) / kTile * kTile;
     p.key_splits = (max_seqlen + p.key_range - 1) / p.key_range;
-    p.row_range = 1024;
-    p.ranges = (p.rows + p.row_range - 1) / p.row_range;
+    p.row_range = kRows;
+    p.ranges = (rows + kRows - 1) / kRows;
+    p.heads = 1;
+    if (p.ranges == 1) {
+        const int64_t padded = (rows + kTile - 1) / kTile * kTile, tiles = (max_seqlen + kHeld - 1) / kHeld;
+        while (p.heads * 2 <= group && p.heads * 2 * padded <= kRows &&
+               tiles * per_group * ((group + p.heads * 2 - 1) / (p.heads * 2)) >= 512)
+            p.heads *= 2;
+    }
+    p.items_h = (group + p.heads - 1) / p.heads;
     return p;
+}
+
+int64_t stats_workgroups(const Plan& p, const PromptWeightsArgs& x) {
+    const int64_t groups = ((x.last + kCols - 1) / kCols * (x.hq / x.hkv) + kWaves - 1) / kWaves;
+    return groups * p.key_splits * x.batch * x.hkv;
+}
+
+int64_t sums_workgroups(const Plan& p, const PromptWeightsArgs& x) {
+    return (x.max_seqlen + kHeld - 1) / kHeld * p.items_h * p.ranges * x.batch * x.hkv;
 }
 
 template <int D, class T>
@@ -359,17 +430,19 @@ hipError_t launch(const PromptWeightsArgs& x) {
     p.length = (int)x.length;
     p.key_range = (int)plan.key_range;
     p.key_splits = (int)plan.key_splits;
+    p.heads = (int)plan.heads;
+    p.items_h = (int)plan.items_h;
     p.row_range = (int)plan.row_range;
     p.ranges = (int)plan.ranges;
     p.sl2 = x.sl2;
+    p.pairs = (int)(x.batch * x.hkv);
+    p.key_tiles = (int)((x.max_seqlen + kHeld - 1) / kHeld);
     const auto stream = (hipStream_t)x.stream;
     const unsigned hkv = (unsigned)x.hkv, batch = (unsigned)x.batch;
-    const int64_t groups = ((plan.rows + kCols - 1) / kCols * p.group + kWaves - 1) / kWaves;
-    hipLaunchKernelGGL((prompt_stats_kernel<D, T>), dim3((unsigned)(groups * plan.key_splits), hkv, batch),
-                       dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((prompt_sums_kernel<D, T>),
-                       dim3((unsigned)((x.max_seqlen + kHeld - 1) / kHeld), (unsigned)(p.group * plan.ranges) * hkv, batch),
-                       dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((prompt_stats_kernel<D, T>), dim3((unsigned)stats_workgroups(plan, x)), dim3(kThreads), 0, stream,
+                       p);
+    hipLaunchKernelGGL((prompt_sums_kernel<D, T>), dim3((unsigned)sums_workgroups(plan, x)), dim3(kThreads), 0, stream,
+                       p);
     hipLaunchKernelGGL(prompt_join_kernel, dim3((unsigned)((x.length + kThreads - 1) / kThreads), hkv, batch),
                        dim3(kThreads), 0, stream, p);
     return hipGetLastError();
@@ -380,7 +453,7 @@ hipError_t launch(const PromptWeightsArgs& x) {
 size_t prompt_weights_workspace(int64_t batch, int64_t total, int64_t hq, int64_t hkv, int64_t max_seqlen,
                                 int64_t last) {
     const Plan p = make_plan(batch, hq, hkv, max_seqlen, last);
-    return sizeof(float) * (size_t)total * (size_t)(2 * p.key_splits * hq + hq * p.ranges);
+    return sizeof(float) * (size_t)total * (size_t)(2 * p.key_splits * hq + hkv * p.items_h * p.ranges);
 }
 
 hipError_t prompt_weights_launch(const PromptWeightsArgs& x) {
@@ -398,6 +471,12 @@ hipError_t prompt_weights_launch(const PromptWeightsArgs& x) {
     }
     if (x.d == 128) return x.bf16 ? launch<128, bf16>(x) : launch<128, f16>(x);
     return x.bf16 ? launch<64, bf16>(x) : launch<64, f16>(x);
+}
+
+bool prompt_weights_fits(const PromptWeightsArgs& x) {
+    if (x.total == 0 || x.max_seqlen == 0) return true;
+    const Plan p = make_plan(x.batch, x.hq, x.hkv, x.max_seqlen, x.last);
+    return std::max(stats_workgroups(p, x), sums_workgroups(p, x)) <= INT32_MAX;
 }
 
 }  // namespace ak

@@ -283,7 +283,7 @@ int ak_paged_decode_weights(const void *q, const void *k_cache, const void *v_ca
  * kv, j] = the sum over the kv head's query heads and over the sequence's last
  * `last` queries i >= j of softmax_j(scale q_i.k_j, j <= i), 0 from the sequence's
  * length on.  q [total_rows, num_heads, head_dim] and k [total_rows, num_kv_heads,
- * head_dim] with token strides in elements (multiples of 8; heads contiguous);
+ * head_dim] with token strides in elements (multiples of 8 up to 2^24; heads contiguous);
  * cu_seqlens and max_seqlen as in ak_prefill_varlen, max_seqlen <= weights_length. */
 size_t ak_prompt_weights_workspace_size(int64_t batch, int64_t total_rows, int64_t num_heads,
                                         int64_t num_kv_heads, int64_t head_dim, int64_t max_seqlen,
