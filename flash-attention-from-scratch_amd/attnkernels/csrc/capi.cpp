@@ -667,7 +667,9 @@ int ak_prompt_weights(const void* q, const void* k, const int32_t* cu_seqlens, f
     a.w_stride_b = weights_stride_b;
     a.w_stride_h = weights_stride_h;
     a.bf16 = bf16 != 0;
-    a.sl2 = (float)(scale * kLog2e);
+    // |scale| * log2(e) is kept >= 1e-30, so that masked scores (infinite) still get no
+    // weight; below that every score weighs the same anyway.
+    a.sl2 = (float)std::copysign(std::fmax(std::fabs(scale) * kLog2e, 1e-30), scale);
     a.stream = stream;
     if (!ak::prompt_weights_fits(a)) return fail(AK_ERR_INVALID_ARGUMENT, "prompt_weights: size out of range");
     return hip_status(ak::prompt_weights_launch(a), who);

@@ -21,7 +21,6 @@
 // the first tile unless a sum passes 2^100: sums are in fp32, whose exponent has
 // room for the rest.
 #include <algorithm>
-#include <type_traits>
 
 #include "attn_kernels.hpp"
 #include "mxfp4.hpp"
@@ -120,6 +119,25 @@ __device__ __forceinline__ void tile_ready(int later) {
     __syncthreads();
 }
 
+// The score that is -infinity once it is scaled.
+__device__ __forceinline__ float masked_score(float sl2) { return sl2 < 0.f ? INFINITY : -INFINITY; }
+
+// The order of a stage's instructions (0x008 MFMA, 0x002 vector, 0x400
+// exponentials, 0x100 LDS reads): the products of one block with an equal share
+// of the other's exponentials and VALU vector instructions behind each.
+template <int D, int VALU>
+__device__ __forceinline__ void interleave() {
+    constexpr int N = D / 8;  // products
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (VALU + N - 1) / N, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 32 / N, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
 // Scores (unscaled) of the tile's rows 32 blk .. 32 blk + 31 against the held columns.
 template <int D, class T>
 __device__ __forceinline__ void product(const u32x4* tile, int blk, const u32x4 (&held)[2][D / 16], int lane,
@@ -176,67 +194,71 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params 
     u32x4 held[2][D / 16];
     hold<D>(queries, q0, sq.n, lane, held);
 
+    const float lowest = masked_score(a.sl2);
     float m[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f};
-    // Adds a tile's exponentials to l.
-    auto add = [&](const u32x4* tile, int k0, auto masked) {
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            const int kb = k0 + 32 * blk;
-            f32x16 s[2];
-            product<D, T>(tile, blk, held, lane, s);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                int limit = min(q0 + 32 * c + (lane & 31), end - 1) - kb;  // the last key that counts
-                if (decltype(masked)::value) asm volatile("" : "+v"(limit));  // not compared ahead of the branch
-                float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float x = s[c][r] * a.sl2 - m[c];
-                    if (decltype(masked)::value) x = row_of(r, lane) > limit ? -INFINITY : x;
-                    t[r % 4] += exp2_fast(x);
-                }
-                l[c] += (t[0] + t[1]) + (t[2] + t[3]);
-            }
-        }
-    };
-    auto raise = [&](const u32x4* tile, int k0) {  // m to the tile's maximum
-        float mx[2] = {m[0], m[1]};
-#pragma unroll 1
-        for (int blk = 0; blk < 2; ++blk) {
-            const int kb = k0 + 32 * blk;
-            f32x16 s[2];
-            product<D, T>(tile, blk, held, lane, s);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int limit = min(q0 + 32 * c + (lane & 31), end - 1) - kb;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx[c] = fmaxf(mx[c], row_of(r, lane) > limit ? kLowest : s[c][r] * a.sl2);
-            }
-        }
+    // Adds the exponentials of a block's scores to sum.
+    auto weigh = [&](const f32x16 (&x)[2], float (&sum)[2]) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            l[c] *= exp2_fast(m[c] - mx[c]);
-            m[c] = mx[c];
+            float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r % 4] += exp2_fast(x[c][r] * a.sl2 - m[c]);
+            sum[c] = l[c] + ((t[0] + t[1]) + (t[2] + t[3]));
         }
     };
+    // One stage: the scores of rows kb .. (tile block blk) into x, while those of
+    // the block before, y, become exponentials; live: the block before has any.
+    bool live = false;
+    auto stage = [&](const u32x4* tile, int blk, int kb, f32x16 (&x)[2], const f32x16 (&y)[2]) {
+        const bool now = !spare && kb < end && kb < q0 + kCols;  // a key that some query sees
+        float sum[2];
+        if (now && live) {
+            product<D, T>(tile, blk, held, lane, x);
+            weigh(y, sum);
+            interleave<D, 32 * 2 + 8>();
+        } else if (now) {
+            product<D, T>(tile, blk, held, lane, x);
+        } else if (live) {
+            weigh(y, sum);
+        }
+        if (live) {
+            // The maximum subtracted stays unless the sums pass 2^100 (as
+            // against the lowest number at first); then the block is done again.
+            if (__builtin_amdgcn_ballot_w64(!(sum[0] <= 0x1p100f) || !(sum[1] <= 0x1p100f))) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float mx = m[c];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[c][r] * a.sl2);
+                    l[c] *= exp2_fast(m[c] - mx);
+                    m[c] = mx;
+                }
+                weigh(y, sum);
+            }
+            l[0] = sum[0];
+            l[1] = sum[1];
+        }
+        if (now && (kb + 31 > q0 || kb + 32 > end)) {  // keys after a query, or past the range
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                int limit = min(q0 + 32 * c + (lane & 31), end - 1) - kb;
+                asm volatile("" : "+v"(limit));  // nothing of this is done ahead of the branch
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[c][r] = row_of(r, lane) > limit ? lowest : x[c][r];
+            }
+        }
+        live = now;
+    };
+    f32x16 x[2], y[2];
     for (int t = 0, cur = 0; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
         const int k0 = begin + t * kTile;
         tile_ready<D>(count - 1 - t);
         if (t + kRing - 1 < count)
             load_tile<D>(keys, k0 + (kRing - 1) * kTile, end, tiles[cur == 0 ? kRing - 1 : cur - 1], w, lane);
-        if (spare || k0 > q0 + kCols - 1) continue;
-        const u32x4* tile = tiles[cur];
-        const float l0 = l[0], l1 = l[1];
-        const bool masked = k0 + kTile - 1 > q0 || k0 + kTile > end;
-        // The maximum subtracted stays unless the sums pass 2^100; then the tile is done again.
-        for (bool again = false;; again = true) {
-            masked ? add(tile, k0, std::true_type{}) : add(tile, k0, std::false_type{});
-            if (again || !__builtin_amdgcn_ballot_w64(!(l[0] <= 0x1p100f) || !(l[1] <= 0x1p100f))) break;
-            l[0] = l0;
-            l[1] = l1;
-            raise(tile, k0);
-        }
+        stage(tiles[cur], 0, k0, x, y);
+        stage(tiles[cur], 1, k0 + 32, y, x);
     }
+    stage(tiles[0], 0, end, x, y);  // the last block's exponentials
     if (spare) return;
     // A column's rows are in two lanes.
 #pragma unroll
@@ -300,10 +322,20 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
             const size_t at = (size_t)(h0 + head) * a.total + sq.start + pos;
             float L = 0.f;
             m = kLowest;
-            for (int p = 0; p < a.key_splits; ++p) {
-                const float lp = a.l[at + p * step], mp = a.m[at + p * step];
-                const float mx = lp == 0.f ? m : fmaxf(m, mp);
-                L = L * exp2_fast(m - mx) + (lp == 0.f ? 0.f : lp * exp2_fast(mp - mx));
+            for (int p0 = 0; p0 < a.key_splits; p0 += 4) {
+                float lp[4], mp[4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {  // the loads of four splits together
+                    const size_t from = at + min(p0 + p, a.key_splits - 1) * step;
+                    lp[p] = p0 + p < a.key_splits ? a.l[from] : 0.f;
+                    mp[p] = a.m[from];
+                }
+                float mx = m;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) mx = lp[p] == 0.f ? mx : fmaxf(mx, mp[p]);
+                L *= exp2_fast(m - mx);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) L += lp[p] == 0.f ? 0.f : lp[p] * exp2_fast(mp[p] - mx);
                 m = mx;
             }
             wgt = L == 0.f ? 0.f : 1.f / L;  // every score -inf: nothing
@@ -311,42 +343,54 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
         reinterpret_cast<float*>(row_m)[i] = m;
         reinterpret_cast<float*>(row_w)[i] = wgt;
     }
+    const float lowest = masked_score(a.sl2);
     float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-    auto add = [&](const u32x4* tile, int t, int i0, auto masked) {
+    // Adds a block's weights; its rows' numbers among row_m and row_w start at 32 at.
+    auto weigh = [&](const f32x16 (&x)[2], int at) {
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            const int ib = i0 + 32 * blk;
-            f32x16 s[2];
-            product<D, T>(tile, blk, held, lane, s);
-            f32x4 m[4], wgt[4];
+        for (int r = 0; r < 16; r += 4) {
+            const f32x4 m = row_m[8 * at + r / 2 + (lane >> 5)], wgt = row_w[8 * at + r / 2 + (lane >> 5)];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                m[r] = row_m[16 * t + 8 * blk + 2 * r + (lane >> 5)];
-                wgt[r] = row_w[16 * t + 8 * blk + 2 * r + (lane >> 5)];
-            }
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                int limit = k0 + 32 * c + (lane & 31) - ib;  // the first query that sees the key
-                if (decltype(masked)::value) asm volatile("" : "+v"(limit));  // not compared ahead of the branch
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float x = s[c][r] * a.sl2 - m[r / 4][r % 4];
-                    if (decltype(masked)::value) x = row_of(r, lane) < limit ? -INFINITY : x;
-                    sum[c][r % 2] = fmaf(exp2_fast(x), wgt[r / 4][r % 4], sum[c][r % 2]);
-                }
-            }
+                for (int i = 0; i < 4; ++i)
+                    sum[c][i % 2] = fmaf(exp2_fast(x[c][r + i] * a.sl2 - m[i]), wgt[i], sum[c][i % 2]);
         }
     };
+    // One stage, as in the first pass: rows ib .. , the at-th block.
+    bool live = false;
+    auto stage = [&](const u32x4* tile, int blk, int ib, int at, f32x16 (&x)[2], const f32x16 (&y)[2]) {
+        const bool now = ib < end && ib + 32 > k0;  // a query that sees some key
+        if (now && live) {
+            product<D, T>(tile, blk, held, lane, x);
+            weigh(y, at - 1);
+            interleave<D, 32 * 2>();
+        } else if (now) {
+            product<D, T>(tile, blk, held, lane, x);
+        } else if (live) {
+            weigh(y, at - 1);
+        }
+        if (now && ib < k0 + kCols - 1) {  // queries before a key
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                int limit = k0 + 32 * c + (lane & 31) - ib;
+                asm volatile("" : "+v"(limit));  // nothing of this is done ahead of the branch
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[c][r] = row_of(r, lane) < limit ? lowest : x[c][r];
+            }
+        }
+        live = now;
+    };
+    f32x16 x[2], y[2];
     for (int t = 0, cur = 0, i0 = begin; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
         tile_ready<D>(count - 1 - t);
         if (t + kRing - 1 < count) load_next(cur == 0 ? kRing - 1 : cur - 1);
-        if (i0 + kTile > k0) {  // else every query is before the wave's keys
-            if (i0 < k0 + kCols - 1) add(tiles[cur], t, i0, std::true_type{});
-            else add(tiles[cur], t, i0, std::false_type{});
-        }
+        stage(tiles[cur], 0, i0, 2 * t, x, y);
+        stage(tiles[cur], 1, i0 + 32, 2 * t + 1, y, x);
         i0 += kTile;
         if (i0 >= end) i0 = begin;
     }
+    stage(tiles[0], 0, end, 2 * count, x, y);  // the last block's weights
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         const float one = sum[c][0] + sum[c][1], both = one + __shfl_xor(one, 32, kWave);
@@ -360,11 +404,16 @@ __global__ void __launch_bounds__(kThreads) prompt_join_kernel(const Params a) {
     if (i >= a.length) return;
     const Sequence sq = sequence(a, b);
     float sum = 0.f;
-    if (i < sq.n)
+    if (i < sq.n) {
+        // The ranges whose queries reach the token's tile are the last ones.
+        const int used = (sq.n - sq.first + a.row_range - 1) / a.row_range, tile = i / kHeld * kHeld;
+        const int j0 = min(max((tile - sq.first) / a.row_range, 0), used);
+        const float* p = a.partial + (size_t)kvh * a.total + sq.start + i;
+        const size_t step = (size_t)a.hkv * a.total;
         for (int item = 0; item < a.items_h; ++item)
-            for (int j = 0; j < a.ranges; ++j)
-                if (reaches(a, sq, j, i / kHeld))
-                    sum += a.partial[((size_t)(item * a.ranges + j) * a.hkv + kvh) * a.total + sq.start + i];
+#pragma unroll 8
+            for (int j = j0; j < used; ++j) sum += p[(item * a.ranges + j) * step];
+    }
     a.weights[b * a.w_stride_b + kvh * a.w_stride_h + i] = sum;
 }
 
@@ -380,8 +429,8 @@ Plan make_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t max_seqlen, int64
     Plan p;
     const int64_t rows = std::min(last, max_seqlen), group = hq / hkv, per_group = batch * hkv;
     const int64_t groups = ((rows + kCols - 1) / kCols * group + kWaves - 1) / kWaves;
-    const int64_t most = (max_seqlen + 255) / 256;  // ranges of at least 256 keys
-    const int64_t want = std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(1, groups * per_group)));
+    const int64_t most = (max_seqlen + 127) / 128;  // ranges of at least 128 keys
+    const int64_t want = std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(1, groups * per_group)));
     p.key_range = ((max_seqlen + want - 1) / want + kTile - 1) / kTile * kTile;
     p.key_splits = (max_seqlen + p.key_range - 1) / p.key_range;
     p.row_range = kRows;
