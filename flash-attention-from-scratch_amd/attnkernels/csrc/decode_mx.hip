@@ -31,6 +31,8 @@
 #include "index_math.hpp"
 #include "mxfp4.hpp"
 
+#include <type_traits>
+
 namespace ak {
 
 namespace {
@@ -129,11 +131,10 @@ struct Tile {
     static constexpr int VW = MX ? 1 : D / 32;        // dwords of a V row's D/16 channels (4 bits, D = 64: half of one)
     uint32_t k[2][KW], v[2][4][VW];
     uint32_t ks[2], vs[2][4];
-    uint32_t valid;                                   // bit i: token t + i is read (wave-uniform)
 };
 
 template <int D, class T, bool MX, bool WEIGHTS>
-__global__ void __launch_bounds__(kThreads) decode_mx_kernel(const Params a) {
+__global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) {
     using Tl = Tile<D, T, MX>;
     constexpr int DPL = D / 16;             // channels of a V row per lane = products per tile
     constexpr int KS = D / 32;              // products of S^T per block
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) decode_mx_kernel(const Params a) {
     }
     const int* bt = a.block_tables + (size_t)b * a.max_blocks;
     const int stride = kWaves * kTile;
-    int t = start + w * kTile;
+    const int t = start + w * kTile;  // the wave's first tile
 
     auto pages = [&](int tile) {  // the page of token tile + lane % 32
         const int tok = tile + (lane & 31);
@@ -178,54 +179,65 @@ __global__ void __launch_bounds__(kThreads) decode_mx_kernel(const Params a) {
         }
     }
 
-    // Loads of one lane from the row of a token (row: counted over the pool).
-    auto load_k = [&](Tl& x, int blk, size_t row) {
-        const char* p = static_cast<const char*>(a.k) + row * KROW;
+    // What a lane loads of a block's rows: byte offsets from the first row of the
+    // block (a scalar base where the block is in one page), V's rows apart.
+    constexpr int SROW = D / 32;  // scales of a row
+    const uint32_t k_off = n * KROW + (MX ? KROW / 4 : 16) * g, v_off = 4 * g * KROW + KROW / 16 * n;
+    const uint32_t ks_off = n * SROW + g / (4 / SROW), vs_off = 4 * g * SROW + n / (16 / SROW);
+    auto load_k = [&](Tl& x, int blk, const char* p, const uint8_t* sc) {
         if constexpr (MX && D == 128) {
-            const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 16 * g));
+            const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
 #pragma unroll
             for (int i = 0; i < 4; ++i) x.k[blk][i] = y[i];
         } else if constexpr (MX) {
             typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + 8 * g));
+            const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
             x.k[blk][0] = y[0];
             x.k[blk][1] = y[1];
         } else {
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 64 * s + 16 * g));
+                const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 64 * s));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x.k[blk][4 * s + i] = y[i];
             }
         }
-        if constexpr (MX) x.ks[blk] = a.k_scales[row * (D / 32) + (D == 128 ? g : g / 2)];
+        if constexpr (MX) x.ks[blk] = *sc;
     };
-    auto load_v = [&](Tl& x, int blk, int r, size_t row) {
-        const char* p = static_cast<const char*>(a.v) + row * KROW;
+    auto load_v = [&](Tl& x, int blk, int r, const char* p, const uint8_t* sc) {
         if constexpr (MX && D == 128) {
-            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p + 4 * n));
+            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
         } else if constexpr (MX) {
-            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p + 2 * n));
+            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p));
         } else {
             typedef uint32_t vec __attribute__((ext_vector_type(Tl::VW)));
-            const vec y = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p + 4 * Tl::VW * n));
+            const vec y = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p));
 #pragma unroll
             for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = y[i];
         }
-        if constexpr (MX) x.vs[blk][r] = a.v_scales[row * (D / 32) + n / 8 * (D / 64) + (D == 128 ? n / 4 % 2 : 0)];
+        if constexpr (MX) x.vs[blk][r] = *sc;
     };
-    auto load = [&](Tl& x, int tile, int pid) {
-        x.valid = (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)pid < (unsigned)a.num_blocks);
-        if (fast_bs && x.valid == 0xffffffffu) {
+    // Starts the loads of a tile's K (with what = 0) or V (1): pid is the page of
+    // the lane's token, valid has a bit for each of the tile's tokens that is read.
+    auto load = [&](Tl& x, int tile, int pid, uint32_t valid, auto what) {
+        constexpr bool V = decltype(what)::value;
+        const char* cache = static_cast<const char*>(V ? a.v : a.k);
+        const uint8_t* scales = V ? a.v_scales : a.k_scales;
+        if (fast_bs && valid == 0xffffffffu) {
             // Each block within one page: two page ids for the wave.
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
                 const int p = __builtin_amdgcn_readlane(pid, 16 * blk), tb = uniform(tile) + 16 * blk;
                 const int in = a.bs_shift >= 0 ? tb & (a.bs - 1) : tb % a.bs;
                 const size_t row = ((size_t)p * a.hkv + kvh) * a.bs + in;
-                load_k(x, blk, row + n);
+                const char* base = cache + row * KROW;
+                const uint8_t* sbase = scales + row * SROW;
+                if constexpr (V) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) load_v(x, blk, r, row + 4 * g + r);
+                    for (int r = 0; r < 4; ++r) load_v(x, blk, r, base + v_off + r * KROW, sbase + vs_off + r * SROW);
+                } else {
+                    load_k(x, blk, base + k_off, sbase + ks_off);
+                }
             }
         } else {
             // Every token's row on its own, as lane (token % 32) knows it; rows
@@ -238,18 +250,25 @@ __global__ void __launch_bounds__(kThreads) decode_mx_kernel(const Params a) {
             };
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
-                x.ks[blk] = 127;
+                if constexpr (V) {
 #pragma unroll
-                for (int i = 0; i < Tl::KW; ++i) x.k[blk][i] = 0;
-                const size_t kr = row_of(16 * blk + n);
-                if (x.valid >> (16 * blk + n) & 1) load_k(x, blk, kr);
+                    for (int r = 0; r < 4; ++r) {
+                        x.vs[blk][r] = 127;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x.vs[blk][r] = 127;
+                        for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = 0;
+                        const int i = 16 * blk + 4 * g + r;
+                        const size_t row = row_of(i);
+                        if (valid >> i & 1)
+                            load_v(x, blk, r, cache + row * KROW + (v_off - 4 * g * KROW),
+                                   scales + row * SROW + (vs_off - 4 * g * SROW));
+                    }
+                } else {
+                    x.ks[blk] = 127;
 #pragma unroll
-                    for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = 0;
-                    const size_t vr = row_of(16 * blk + 4 * g + r);
-                    if (x.valid >> (16 * blk + 4 * g + r) & 1) load_v(x, blk, r, vr);
+                    for (int i = 0; i < Tl::KW; ++i) x.k[blk][i] = 0;
+                    const size_t row = row_of(16 * blk + n);
+                    if (valid >> (16 * blk + n) & 1)
+                        load_k(x, blk, cache + row * KROW + (k_off - n * KROW), scales + row * SROW + (ks_off - n * SROW));
                 }
             }
         }
@@ -263,113 +282,123 @@ __global__ void __launch_bounds__(kThreads) decode_mx_kernel(const Params a) {
     for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float* scores = WEIGHTS ? a.scores + (row0 + (n < G ? n : 0)) * a.scores_stride + 4 * g : nullptr;
 
-    auto step = [&](const Tl& x, int tile) {
-        f32x4 s[2];
+    // The tiles of the wave.  A tile's K registers take the next tile's loads as
+    // soon as its scores are formed, its V registers once they are converted.
+    Tl x;
+    f32x4 s[2];
+    uint32_t valid = 0;
+    int next = pages(t);  // the next tile's pages
+    for (int tile = t - stride, tn = t;; tile = tn, tn += stride) {
+        const bool now = tile >= start, more = tn < end;  // tiles before tn are all in the split
+        const int pid = next;
+        next = pages(tn + stride);
+        const uint32_t valid_next = (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)pid < (unsigned)a.num_blocks);
+        if (now) {
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-            s[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int blk = 0; blk < 2; ++blk) {
+                s[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                u32x4 kf;
-                if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], mx_scale(x.ks[blk]));
-                else kf = u32x4{x.k[blk][4 * i], x.k[blk][4 * i + 1], x.k[blk][4 * i + 2], x.k[blk][4 * i + 3]};
-                s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
+                for (int i = 0; i < KS; ++i) {
+                    u32x4 kf;
+                    if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], mx_scale(x.ks[blk]));
+                    else kf = u32x4{x.k[blk][4 * i], x.k[blk][4 * i + 1], x.k[blk][4 * i + 2], x.k[blk][4 * i + 3]};
+                    s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
+                }
             }
+        }
+        if (more) load(x, tn, pid, valid_next, std::false_type{});
+        if (now) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[blk][r] *= a.sl2;
-            if (x.valid != 0xffffffffu) {
+            for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    s[blk][r] = x.valid >> (16 * blk + 4 * g + r) & 1 ? s[blk][r] : -INFINITY;
+                for (int r = 0; r < 4; ++r) s[blk][r] *= a.sl2;
+            if (valid != 0xffffffffu) {
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[blk][r] = valid >> (16 * blk + 4 * g + r) & 1 ? s[blk][r] : -INFINITY;
             }
             if constexpr (WEIGHTS) {
-                if (n < G) *reinterpret_cast<f32x4*>(scores + tile + 16 * blk) = s[blk];
+                if (n < G) {
+                    *reinterpret_cast<f32x4*>(scores + tile) = s[0];
+                    *reinterpret_cast<f32x4*>(scores + tile + 16) = s[1];
+                }
             }
-        }
-        float p[8];
-        bool ok = true;
+            float p[8];
+            bool ok = true;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
-            ok = ok && p[i] <= kPMax;
-        }
-        if (__builtin_amdgcn_ballot_w64(!ok)) {
-            // Move the reference maximum of every head to its running maximum.
-            float mx = m_own;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-            const float alpha = exp2_fast(m_own - mx);
-            l_own *= alpha;
-            m_own = mx;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {  // accumulator row r is head 4g + r
-                const float al = __shfl(alpha, 4 * g + r, kWave);
-#pragma unroll
-                for (int j = 0; j < DPL; ++j) acc[j][r] *= al;
+            for (int i = 0; i < 8; ++i) {
+                p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+                ok = ok && p[i] <= kPMax;
             }
+            if (__builtin_amdgcn_ballot_w64(!ok)) {
+                // Move the reference maximum of every head to its running maximum.
+                float mx = m_own;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
-        }
-        l_own += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        u32x4 pf;
+                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+                mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+                const float alpha = exp2_fast(m_own - mx);
+                l_own *= alpha;
+                m_own = mx;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pf[i] = Half<T>::pack(p[2 * i], p[2 * i + 1]);
-        // V: the lane's channels of its eight tokens, two tokens to a register.
-        uint32_t vr[8][DPL / 2];
+                for (int r = 0; r < 4; ++r) {  // accumulator row r is head 4g + r
+                    const float al = __shfl(alpha, 4 * g + r, kWave);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+                    for (int j = 0; j < DPL; ++j) acc[j][r] *= al;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+            }
+            l_own += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            u32x4 pf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pf[i] = Half<T>::pack(p[2 * i], p[2 * i + 1]);
+            // V: channels 2c, 2c + 1 of the lane's eight tokens, paired by tokens.
+            auto channels = [&](const uint32_t (&v)[8], int c) {
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                    const uint32_t sel = o ? 0x07060302u : 0x05040100u;
+                    u32x4 f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], sel);
+                    acc[2 * c + o] = Half<T>::mfma(pf, f, acc[2 * c + o]);
+                }
+            };
             if constexpr (MX) {
-                const float sc = mx_scale(x.vs[i / 4][i % 4]);
-                const uint32_t c = x.v[i / 4][i % 4][0];
-                vr[i][0] = Half<T>::template decode<0>(c, sc);
-                vr[i][1] = Half<T>::template decode<1>(c, sc);
+                uint32_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = Half<T>::template decode<0>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
+                channels(v, 0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = Half<T>::template decode<1>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
+                channels(v, 1);
                 if constexpr (DPL == 8) {
-                    vr[i][2] = Half<T>::template decode<2>(c, sc);
-                    vr[i][3] = Half<T>::template decode<3>(c, sc);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        v[i] = Half<T>::template decode<2>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
+                    channels(v, 2);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        v[i] = Half<T>::template decode<3>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
+                    channels(v, 3);
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < DPL / 2; ++j) vr[i][j] = x.v[i / 4][i % 4][j];
-            }
-        }
+                for (int c = 0; c < DPL / 2; ++c) {
+                    uint32_t v[8];
 #pragma unroll
-        for (int j = 0; j < DPL; ++j) {
-            const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-            u32x4 f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][j / 2], vr[2 * i][j / 2], sel);
-            acc[j] = Half<T>::mfma(pf, f, acc[j]);
-        }
-    };
-
-    if (t < end) {
-        int pid = pages(t), next = pages(t + stride);
-        if constexpr (MX) {  // the next tile's rows are on their way while this one is computed
-            Tl x, y;
-            load(x, t, pid);
-            while (true) {
-                const int t1 = t + stride, t2 = t1 + stride;
-                pid = pages(t2);
-                if (t1 < end) load(y, t1, next);
-                step(x, t);
-                if (t1 >= end) break;
-                next = pages(t2 + stride);
-                if (t2 < end) load(x, t2, pid);
-                step(y, t1);
-                if (t2 >= end) break;
-                t = t2;
-            }
-        } else {
-            for (; t < end; t += stride) {
-                Tl x;
-                load(x, t, pid);
-                pid = next;
-                next = pages(t + 2 * stride);
-                step(x, t);
+                    for (int i = 0; i < 8; ++i) v[i] = x.v[i / 4][i % 4][c];
+                    channels(v, c);
+                }
             }
         }
+        if (!more) break;
+        load(x, tn, pid, valid_next, std::true_type{});
+        valid = valid_next;
     }
 
     // Merge: l over the four lanes of each head, then the waves through LDS.
