@@ -119,12 +119,6 @@ __device__ __forceinline__ void merge_row(const Params& a, size_t row, int ns, f
     }
 }
 
-// Where a lane's tokens are read: pages of the tile's tokens, one per lane (token
-// t + lane % 32), -1 where there is none.
-__device__ __forceinline__ int page_index(int t, const Params& a) {
-    return a.bs_shift >= 0 ? t >> a.bs_shift : t / a.bs;
-}
-
 template <int D, class T, bool MX>
 struct Tile {
     static constexpr int KW = MX ? D / 32 : D / 8;    // dwords of K per block: a quarter row
@@ -160,13 +154,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     }
     const int* bt = a.block_tables + (size_t)b * a.max_blocks;
     const int stride = kWaves * kTile;
-    const int t = start + w * kTile;  // the wave's first tile
-
-    auto pages = [&](int tile) {  // the page of token tile + lane % 32
-        const int tok = tile + (lane & 31);
-        return tok < end ? bt[page_index(tok, a)] : -1;
-    };
-    const bool fast_bs = a.bs % 16 == 0;
+    int t = start + w * kTile;
 
     // Q^T: head n (zeros past the group), the channels that the lane's K holds.
     u32x4 qf[KS];
@@ -179,11 +167,12 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
         }
     }
 
-    // What a lane loads of a block's rows: byte offsets from the first row of the
-    // block (a scalar base where the block is in one page), V's rows apart.
-    constexpr int SROW = D / 32;  // scales of a row
+    // What a lane loads of a block's rows: byte offsets from the block's first
+    // row.  Of the scales it loads a row's (4 or 2 bytes) and shifts its group's.
+    constexpr int SROW = D / 32;
+    typedef std::conditional_t<D == 128, uint32_t, uint16_t> scales_t;
     const uint32_t k_off = n * KROW + (MX ? KROW / 4 : 16) * g, v_off = 4 * g * KROW + KROW / 16 * n;
-    const uint32_t ks_off = n * SROW + g / (4 / SROW), vs_off = 4 * g * SROW + n / (16 / SROW);
+    const uint32_t k_shift = g / (4 / SROW) * 8, v_shift = n / (16 / SROW) * 8;
     auto load_k = [&](Tl& x, int blk, const char* p, const uint8_t* sc) {
         if constexpr (MX && D == 128) {
             const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
@@ -202,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
                 for (int i = 0; i < 4; ++i) x.k[blk][4 * s + i] = y[i];
             }
         }
-        if constexpr (MX) x.ks[blk] = *sc;
+        if constexpr (MX) x.ks[blk] = *reinterpret_cast<const scales_t*>(sc);
     };
     auto load_v = [&](Tl& x, int blk, int r, const char* p, const uint8_t* sc) {
         if constexpr (MX && D == 128) {
@@ -215,63 +204,61 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
 #pragma unroll
             for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = y[i];
         }
-        if constexpr (MX) x.vs[blk][r] = *sc;
+        if constexpr (MX) x.vs[blk][r] = *reinterpret_cast<const scales_t*>(sc);
     };
-    // Starts the loads of a tile's K (with what = 0) or V (1): pid is the page of
-    // the lane's token, valid has a bit for each of the tile's tokens that is read.
-    auto load = [&](Tl& x, int tile, int pid, uint32_t valid, auto what) {
+    auto group_scale = [](uint32_t word, uint32_t shift) { return mx_scale(word >> shift & 255u); };
+    // A tile each of whose two blocks is in one page: K's or V's loads at scalar
+    // bases, pa and pb the pages.
+    auto load_whole = [&](Tl& x, int tile, int pa, int pb, auto what) {
         constexpr bool V = decltype(what)::value;
         const char* cache = static_cast<const char*>(V ? a.v : a.k);
         const uint8_t* scales = V ? a.v_scales : a.k_scales;
-        if (fast_bs && valid == 0xffffffffu) {
-            // Each block within one page: two page ids for the wave.
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk) {
-                const int p = __builtin_amdgcn_readlane(pid, 16 * blk), tb = uniform(tile) + 16 * blk;
-                const int in = a.bs_shift >= 0 ? tb & (a.bs - 1) : tb % a.bs;
-                const size_t row = ((size_t)p * a.hkv + kvh) * a.bs + in;
-                const char* base = cache + row * KROW;
-                const uint8_t* sbase = scales + row * SROW;
-                if constexpr (V) {
+        for (int blk = 0; blk < 2; ++blk) {
+            const size_t row = ((size_t)(blk ? pb : pa) * a.hkv + kvh) * a.bs + ((tile + 16 * blk) & (a.bs - 1));
+            const char* base = cache + row * KROW;
+            const uint8_t* sbase = scales + row * SROW;
+            if constexpr (V) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) load_v(x, blk, r, base + v_off + r * KROW, sbase + vs_off + r * SROW);
-                } else {
-                    load_k(x, blk, base + k_off, sbase + ks_off);
-                }
-            }
-        } else {
-            // Every token's row on its own, as lane (token % 32) knows it; rows
-            // that are not read are zeros.
-            const int tok = tile + (lane & 31);
-            const int in = a.bs_shift >= 0 ? tok & (a.bs - 1) : tok % a.bs;
-            auto row_of = [&](int i) {
-                const int p = __shfl(pid, i, kWave), o = __shfl(in, i, kWave);
-                return ((size_t)p * a.hkv + kvh) * a.bs + o;
-            };
-#pragma unroll
-            for (int blk = 0; blk < 2; ++blk) {
-                if constexpr (V) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        x.vs[blk][r] = 127;
-#pragma unroll
-                        for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = 0;
-                        const int i = 16 * blk + 4 * g + r;
-                        const size_t row = row_of(i);
-                        if (valid >> i & 1)
-                            load_v(x, blk, r, cache + row * KROW + (v_off - 4 * g * KROW),
-                                   scales + row * SROW + (vs_off - 4 * g * SROW));
-                    }
-                } else {
-                    x.ks[blk] = 127;
-#pragma unroll
-                    for (int i = 0; i < Tl::KW; ++i) x.k[blk][i] = 0;
-                    const size_t row = row_of(16 * blk + n);
-                    if (valid >> (16 * blk + n) & 1)
-                        load_k(x, blk, cache + row * KROW + (k_off - n * KROW), scales + row * SROW + (ks_off - n * SROW));
-                }
+                for (int r = 0; r < 4; ++r)
+                    load_v(x, blk, r, base + v_off + r * KROW, sbase + (uint32_t)(4 * g * SROW) + r * SROW);
+            } else {
+                load_k(x, blk, base + k_off, sbase + (uint32_t)(n * SROW));
             }
         }
+    };
+    // Any tile: every token's row on its own; rows that are not read are zeros.
+    // Returns a bit for each token that is read.
+    auto load_rows = [&](Tl& x, int tile) {
+        const int tok = tile + (lane & 31);
+        const int index = a.bs_shift >= 0 ? tok >> a.bs_shift : tok / a.bs, in = tok - index * a.bs;
+        const int pid = tok < end ? bt[index] : -1;
+        const uint32_t valid = (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)pid < (unsigned)a.num_blocks);
+        auto row_of = [&](int i) {
+            const int p = __shfl(pid, i, kWave), o = __shfl(in, i, kWave);
+            return ((size_t)p * a.hkv + kvh) * a.bs + o;
+        };
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            x.ks[blk] = 0;
+#pragma unroll
+            for (int i = 0; i < Tl::KW; ++i) x.k[blk][i] = 0;
+            const size_t kr = row_of(16 * blk + n);
+            if (valid >> (16 * blk + n) & 1)
+                load_k(x, blk, static_cast<const char*>(a.k) + kr * KROW + (k_off - n * KROW), a.k_scales + kr * SROW);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x.vs[blk][r] = 0;
+#pragma unroll
+                for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = 0;
+                const int i = 16 * blk + 4 * g + r;
+                const size_t vr = row_of(i);
+                if (valid >> i & 1)
+                    load_v(x, blk, r, static_cast<const char*>(a.v) + vr * KROW + (v_off - 4 * g * KROW),
+                           a.v_scales + vr * SROW);
+            }
+        }
+        return valid;
     };
 
     // Reference maximum of head n (the same in its four lanes), this lane's
@@ -282,123 +269,138 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float* scores = WEIGHTS ? a.scores + (row0 + (n < G ? n : 0)) * a.scores_stride + 4 * g : nullptr;
 
-    // The tiles of the wave.  A tile's K registers take the next tile's loads as
-    // soon as its scores are formed, its V registers once they are converted.
-    Tl x;
-    f32x4 s[2];
-    uint32_t valid = 0;
-    int next = pages(t);  // the next tile's pages
-    for (int tile = t - stride, tn = t;; tile = tn, tn += stride) {
-        const bool now = tile >= start, more = tn < end;  // tiles before tn are all in the split
-        const int pid = next;
-        next = pages(tn + stride);
-        const uint32_t valid_next = (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)pid < (unsigned)a.num_blocks);
-        if (now) {
+    // One tile.  after_k and after_v run once the registers of its K, its V are free.
+    auto step = [&](const Tl& x, int tile, uint32_t valid, auto masked, auto after_k, auto after_v) {
+        f32x4 s[2];
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk) {
-                s[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int blk = 0; blk < 2; ++blk) {
+            s[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    u32x4 kf;
-                    if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], mx_scale(x.ks[blk]));
-                    else kf = u32x4{x.k[blk][4 * i], x.k[blk][4 * i + 1], x.k[blk][4 * i + 2], x.k[blk][4 * i + 3]};
-                    s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
-                }
+            for (int i = 0; i < KS; ++i) {
+                u32x4 kf;
+                if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], group_scale(x.ks[blk], k_shift));
+                else kf = u32x4{x.k[blk][4 * i], x.k[blk][4 * i + 1], x.k[blk][4 * i + 2], x.k[blk][4 * i + 3]};
+                s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
             }
         }
-        if (more) load(x, tn, pid, valid_next, std::false_type{});
-        if (now) {
+        after_k();
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk)
+        for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[blk][r] *= a.sl2;
-            if (valid != 0xffffffffu) {
-#pragma unroll
-                for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        s[blk][r] = valid >> (16 * blk + 4 * g + r) & 1 ? s[blk][r] : -INFINITY;
+            for (int r = 0; r < 4; ++r) {
+                s[blk][r] *= a.sl2;
+                if (decltype(masked)::value) s[blk][r] = valid >> (16 * blk + 4 * g + r) & 1 ? s[blk][r] : -INFINITY;
             }
-            if constexpr (WEIGHTS) {
-                if (n < G) {
-                    *reinterpret_cast<f32x4*>(scores + tile) = s[0];
-                    *reinterpret_cast<f32x4*>(scores + tile + 16) = s[1];
-                }
+        if constexpr (WEIGHTS) {
+            if (n < G) {
+                *reinterpret_cast<f32x4*>(scores + tile) = s[0];
+                *reinterpret_cast<f32x4*>(scores + tile + 16) = s[1];
             }
-            float p[8];
-            bool ok = true;
+        }
+        float p[8];
+        bool ok = true;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
-                ok = ok && p[i] <= kPMax;
+        for (int i = 0; i < 8; ++i) {
+            p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+            ok = ok && p[i] <= kPMax;
+        }
+        if (__builtin_amdgcn_ballot_w64(!ok)) {
+            // Move the reference maximum of every head to its running maximum.
+            float mx = m_own;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+            const float alpha = exp2_fast(m_own - mx);
+            l_own *= alpha;
+            m_own = mx;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {  // accumulator row r is head 4g + r
+                const float al = __shfl(alpha, 4 * g + r, kWave);
+#pragma unroll
+                for (int j = 0; j < DPL; ++j) acc[j][r] *= al;
             }
-            if (__builtin_amdgcn_ballot_w64(!ok)) {
-                // Move the reference maximum of every head to its running maximum.
-                float mx = m_own;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
-                mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-                const float alpha = exp2_fast(m_own - mx);
-                l_own *= alpha;
-                m_own = mx;
+            for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+        }
+        l_own += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        u32x4 pf;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {  // accumulator row r is head 4g + r
-                    const float al = __shfl(alpha, 4 * g + r, kWave);
+        for (int i = 0; i < 4; ++i) pf[i] = Half<T>::pack(p[2 * i], p[2 * i + 1]);
+        // V: channels 2c, 2c + 1 of the lane's eight tokens, paired by tokens.
+        auto channels = [&](const uint32_t (&v)[8], int c) {
 #pragma unroll
-                    for (int j = 0; j < DPL; ++j) acc[j][r] *= al;
-                }
+            for (int o = 0; o < 2; ++o) {
+                const uint32_t sel = o ? 0x07060302u : 0x05040100u;
+                u32x4 f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+                for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], sel);
+                acc[2 * c + o] = Half<T>::mfma(pf, f, acc[2 * c + o]);
             }
-            l_own += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            u32x4 pf;
+        };
+        if constexpr (MX) {
+            float sc[8];
+            uint32_t v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pf[i] = Half<T>::pack(p[2 * i], p[2 * i + 1]);
-            // V: channels 2c, 2c + 1 of the lane's eight tokens, paired by tokens.
-            auto channels = [&](const uint32_t (&v)[8], int c) {
+            for (int i = 0; i < 8; ++i) sc[i] = group_scale(x.vs[i / 4][i % 4], v_shift);
 #pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    const uint32_t sel = o ? 0x07060302u : 0x05040100u;
-                    u32x4 f;
+            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<0>(x.v[i / 4][i % 4][0], sc[i]);
+            channels(v, 0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], sel);
-                    acc[2 * c + o] = Half<T>::mfma(pf, f, acc[2 * c + o]);
-                }
-            };
-            if constexpr (MX) {
+            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<1>(x.v[i / 4][i % 4][0], sc[i]);
+            channels(v, 1);
+            if constexpr (DPL == 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<2>(x.v[i / 4][i % 4][0], sc[i]);
+                channels(v, 2);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<3>(x.v[i / 4][i % 4][0], sc[i]);
+                channels(v, 3);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < DPL / 2; ++c) {
                 uint32_t v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = Half<T>::template decode<0>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
-                channels(v, 0);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = Half<T>::template decode<1>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
-                channels(v, 1);
-                if constexpr (DPL == 8) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        v[i] = Half<T>::template decode<2>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
-                    channels(v, 2);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        v[i] = Half<T>::template decode<3>(x.v[i / 4][i % 4][0], mx_scale(x.vs[i / 4][i % 4]));
-                    channels(v, 3);
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < DPL / 2; ++c) {
-                    uint32_t v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = x.v[i / 4][i % 4][c];
-                    channels(v, c);
-                }
+                for (int i = 0; i < 8; ++i) v[i] = x.v[i / 4][i % 4][c];
+                channels(v, c);
             }
         }
-        if (!more) break;
-        load(x, tn, pid, valid_next, std::true_type{});
-        valid = valid_next;
+        after_v();
+    };
+
+    // The wave's tiles.  While they are whole, a tile's K and V registers take the
+    // next tile's loads as soon as they are free, and page ids come a tile earlier.
+    Tl x;
+    bool loaded = false;
+    if (a.bs_shift >= 4) {
+        auto page = [&](int tok) { return tok < end ? bt[uniform(tok >> a.bs_shift)] : -1; };
+        auto whole = [&](int tile, int pa, int pb) {
+            return tile + kTile <= end && (unsigned)pa < (unsigned)a.num_blocks && (unsigned)pb < (unsigned)a.num_blocks;
+        };
+        int pa = page(t), pb = page(t + 16);
+        if (whole(t, pa, pb)) {
+            load_whole(x, t, pa, pb, std::false_type{});
+            load_whole(x, t, pa, pb, std::true_type{});
+            loaded = true;
+            pa = page(t + stride);
+            pb = page(t + stride + 16);
+            while (whole(t + stride, pa, pb)) {
+                const int tn = t + stride, na = page(tn + stride), nb = page(tn + stride + 16);
+                step(x, t, 0xffffffffu, std::false_type{}, [&] { load_whole(x, tn, pa, pb, std::false_type{}); },
+                     [&] { load_whole(x, tn, pa, pb, std::true_type{}); });
+                pa = na;
+                pb = nb;
+                t = tn;
+            }
+        }
+    }
+    // The last whole tile, and the rest: the context's end, pages outside the pool
+    // or of other sizes.
+    for (; t < end; t += stride) {
+        const uint32_t valid = loaded ? 0xffffffffu : load_rows(x, t);
+        loaded = false;
+        step(x, t, valid, std::true_type{}, [] {}, [] {});
     }
 
     // Merge: l over the four lanes of each head, then the waves through LDS.
