@@ -99,13 +99,14 @@ struct DecodeMxArgs {
     const int32_t* block_tables;  // [B, max_blocks]
     const int32_t* context_lens;  // [B]
     void* out;             // [B, hq, D], q's type
-    float* o_part;         // [B, hq, S, D]  split partials
-    float* m_part;         // [B, hq, S]
-    float* l_part;         // [B, hq, S]
+    float* o_part;         // [hq, slots, D]  split partials
+    float* m_part;         // [hq, slots]
+    float* l_part;         // [hq, slots]
     float* scores;         // [B, hq, scores_stride]: scale * log2(e) * q.k, where weights are wanted
     float* weights;        // [B, hkv, >= max_ctx], strides in elements below
     int32_t* counters;     // one per (sequence, kv head), zero on entry and left zero
-    int64_t batch, hq, hkv, d, num_blocks, bs, max_blocks, max_ctx, partition, num_splits;
+    int64_t batch, hq, hkv, d, num_blocks, bs, max_blocks, max_ctx;
+    int64_t partition, slots;  // tokens per split, 0: cut evenly; splits of a kv head over the batch (decode_mx_slots)
     int64_t scores_stride, w_stride_b, w_stride_h;
     bool bf16;
     float sl2;             // scale * log2(e)
@@ -115,8 +116,7 @@ struct DecodeMxArgs {
 hipError_t cache_write_mxfp4_launch(const CacheMxArgs& a);
 hipError_t cache_read_mxfp4_launch(const CacheMxArgs& a);
 hipError_t decode_mx_launch(const DecodeMxArgs& a);
-// Tokens per split where the caller leaves them to the library: a multiple of 256.
-int64_t decode_mx_partition(int64_t batch, int64_t hkv, int64_t max_ctx);
+int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition);
 
 // Eviction by accumulated weight (evict.hip).
 struct EvictArgs {

@@ -212,8 +212,8 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
     const std::string who(name);
     if (num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0)
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": num_heads must be a multiple of num_kv_heads");
-    if (partition <= 0 || partition % kChunk != 0)
-        return fail(AK_ERR_INVALID_ARGUMENT, who + ": partition size must be a positive multiple of 256");
+    if (partition < 0 || partition % kChunk != 0)
+        return fail(AK_ERR_INVALID_ARGUMENT, who + ": partition size must be 0 or a positive multiple of 256");
     if ((head_dim != 64 && head_dim != 128) || num_heads / num_kv_heads > 16)
         return fail(AK_ERR_UNSUPPORTED, who + ": head_dim must be 64 or 128 and num_heads / num_kv_heads at most 16");
     if (batch < 0 || num_blocks < 0 || block_size <= 0 || max_blocks_per_seq < 0)
@@ -233,8 +233,8 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
     if (max_context_len > INT_MAX / 2 || partition > INT_MAX / 2 || num_blocks > INT_MAX ||
         max_blocks_per_seq > INT_MAX / 2 / block_size || batch > 65535 || num_kv_heads > 65535)
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": size out of range");
-    const int64_t splits = (max_context_len + partition - 1) / partition;
-    if (splits > 65535) return fail(AK_ERR_INVALID_ARGUMENT, who + ": more than 65535 splits");
+    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition);
+    if (slots > INT_MAX / num_kv_heads) return fail(AK_ERR_INVALID_ARGUMENT, who + ": too many splits");
     if (weights) {
         if (w_length < max_context_len)
             return fail(AK_ERR_INVALID_ARGUMENT, who + ": weights are shorter than max_context_len");
@@ -243,8 +243,8 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
     if (counters && counters_len < batch * num_kv_heads)
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": counters must be an int32 array of at least batch * num_kv_heads "
                                                    "elements");
-    const size_t need = ak_paged_decode_mx_workspace_size(batch, num_heads, head_dim, max_context_len, partition,
-                                                          weights != nullptr);
+    const size_t need = ak_paged_decode_mx_workspace_size(batch, num_heads, num_kv_heads, head_dim, max_context_len,
+                                                          partition, weights != nullptr);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(AK_ERR_WORKSPACE, who + ": workspace of " + std::to_string(need) + " bytes required, got " +
                                           std::to_string(workspace_bytes));
@@ -269,20 +269,20 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
     a.max_blocks = max_blocks_per_seq;
     a.max_ctx = max_context_len;
     a.partition = partition;
-    a.num_splits = splits;
+    a.slots = slots;
     a.w_stride_b = w_stride_b;
     a.w_stride_h = w_stride_h;
     a.bf16 = bf16 != 0;
     a.sl2 = (float)(scale * kLog2e);
     a.stream = stream;
     if (need > 0) {
-        const size_t rows = (size_t)(batch * num_heads * splits);
+        const size_t rows = (size_t)(num_heads * slots);
         a.o_part = static_cast<float*>(workspace);
         a.m_part = a.o_part + rows * (size_t)head_dim;
         a.l_part = a.m_part + rows;
         if (weights) {
             a.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                                round16(partials_bytes(batch, num_heads, splits, head_dim)));
+                                                round16(partials_bytes(1, num_heads, slots, head_dim)));
             a.scores_stride = scores_row(max_context_len);
         }
     }
@@ -556,19 +556,14 @@ int ak_gather_cache_mxfp4(const void* k_cache, const void* k_scales, const void*
     return hip_status(ak::cache_read_mxfp4_launch(a), who);
 }
 
-int64_t ak_paged_decode_mx_partition(int64_t batch, int64_t num_kv_heads, int64_t max_context_len) {
-    if (batch < 1 || num_kv_heads < 1 || max_context_len < 1 || max_context_len > INT_MAX / 2) return kChunk;
-    return ak::decode_mx_partition(batch, num_kv_heads, max_context_len);
-}
-
-size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64_t head_dim, int64_t max_context_len,
-                                         int64_t partition, int with_weights) {
-    if (batch < 0 || num_heads < 0 || head_dim <= 0 || max_context_len < 1 || partition <= 0 ||
+size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                         int64_t max_context_len, int64_t partition, int with_weights) {
+    if (batch < 1 || num_heads < 1 || num_kv_heads < 1 || head_dim <= 0 || max_context_len < 1 || partition < 0 ||
         max_context_len > INT_MAX / 2)
         return 0;
-    const int64_t splits = (max_context_len + partition - 1) / partition;
-    if (splits <= 1 && !with_weights) return 0;
-    const size_t parts = partials_bytes(batch, num_heads, splits, head_dim);
+    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition);
+    if (slots <= batch && !with_weights) return 0;
+    const size_t parts = partials_bytes(1, num_heads, slots, head_dim);
     return with_weights ? round16(parts) + (size_t)batch * (size_t)num_heads * (size_t)scores_row(max_context_len) *
                                                sizeof(float)
                         : parts;

@@ -22,13 +22,14 @@
 //     loads them row by row and pairs the tokens with v_perm.
 //   * exp2 against a reference maximum that moves only when a score exceeds it
 //     by more than 8, sums in fp32.
-// With weights, the scores (scale * log2 e * q.k in fp32) go to a workspace, and
+// The splits are cut by the kernel from the context lengths, of about equal size
+// over the batch, unless the caller gives a size; the last split of a (sequence,
+// kv head) to finish merges them.  With weights, the scores (scale * log2 e * q.k in fp32) go to a workspace, and
 // a second kernel, which knows every split's maximum and sum, turns them into
 // weights while it merges the splits' outputs.
 #include <algorithm>
 
 #include "attn_kernels.hpp"
-#include "index_math.hpp"
 #include "mxfp4.hpp"
 
 #include <type_traits>
@@ -40,7 +41,9 @@ namespace {
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kTile = 32;           // tokens per wave iteration
 constexpr int kMaxGroup = 16;       // query heads per kv head: rows of the MFMA
-constexpr int kFinishTokens = 1024; // tokens per workgroup of the finishing kernel
+constexpr int kFinishTokens = 512;  // tokens per workgroup of the finishing kernel: two of a thread
+constexpr int kCut = kWaves * kTile; // splits start at multiples of it
+constexpr int kMinSplit = 256;
 constexpr float kLowest = -3.402823466e38f;
 
 struct Params {
@@ -51,7 +54,9 @@ struct Params {
     float *o_part, *m_part, *l_part, *scores, *weights;
     int32_t* counters;
     int64_t scores_stride, w_stride_b, w_stride_h;
-    int hkv, group, bs, bs_shift, max_blocks, num_blocks, max_tok, partition, num_splits;
+    int batch, hkv, group, bs, bs_shift, max_blocks, num_blocks, max_tok;
+    int partition;  // tokens per split; 0: cut evenly
+    int slots;      // splits of a kv head over the whole batch, at most
     float sl2;
 };
 
@@ -62,60 +67,146 @@ __device__ __forceinline__ float coherent_load(const float* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, kWave));
-    return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) x += __shfl_xor(x, m, kWave);
-    return x;
+__device__ __forceinline__ f32x4 coherent_load4(const float* p) {  // 8-byte aligned
+    const uint64_t a = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    const uint64_t b = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p) + 1, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    const f32x2 x = __builtin_bit_cast(f32x2, a), y = __builtin_bit_cast(f32x2, b);
+    return f32x4{x[0], x[1], y[0], y[1]};
 }
 
-// The running maximum m and sum l of one query row over its ns splits, by one
-// wave: split s starts at mp[s], lp[s].  Splits without weight (l = 0) count
-// nothing; a row without any has l = 0.
-__device__ __forceinline__ void merge_stats(const float* mp, const float* lp, int ns, int lane, float& m, float& l) {
+// How a context is cut: ns splits (at least one) of `piece` tokens, the last one
+// shorter.
+struct Cut {
+    int ns, piece;
+};
+__device__ __forceinline__ Cut cut_context(int len, int size) {
+    const int n = max((len + size - 1) / size, 1);
+    Cut c;
+    c.piece = max(((len + n - 1) / n + kCut - 1) / kCut * kCut, kCut);
+    c.ns = max((len + c.piece - 1) / c.piece, 1);
+    return c;
+}
+
+__device__ __forceinline__ int context(const Params& a, int b) { return max(min(a.ctx_lens[b], a.max_tok), 0); }
+
+// Tokens per split.  Cut evenly: so many that the splits of all sequences fit the
+// slots: sum ceil(len / size) <= sum len / size + batch.
+__device__ __forceinline__ int split_size(const Params& a, int lane) {
+    if (a.partition > 0) return a.partition;
+    if (a.slots <= a.batch) return INT32_MAX / 4 / kCut * kCut;  // a split each
+    float total = 0.f;  // off by up to a few thousand units in the last place, which the factor below covers
+    for (int b = lane; b < a.batch; b += kWave) total += (float)context(a, b);
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
+    const float size = total * 1.0005f / (float)(a.slots - a.batch) + 1.f;
+    return max(((int)size + kCut) / kCut * kCut, kMinSplit);
+}
+
+// The split that slot `slot` holds, or slot 0 of sequence `of` (slot < 0): every
+// wave counts the splits of the sequences in order.  b < 0: none.
+struct Segment {
+    int b, split, ns, piece, first, ctx;  // first: the sequence's first slot
+};
+__device__ __forceinline__ Segment segment(const Params& a, int slot, int of, int lane) {
+    Segment s;
+    s.b = -1;
+    const int size = split_size(a, lane);
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+        const int b = b0 + lane, ctx = b < a.batch ? context(a, b) : 0;
+        const Cut c = cut_context(ctx, size);
+        int sum = b < a.batch ? c.ns : 0;  // inclusive
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) {
+            const int y = __shfl_up(sum, d, kWave);
+            if (lane >= d) sum += y;
+        }
+        const uint64_t here = __builtin_amdgcn_ballot_w64(slot >= 0 ? before + sum > slot : b == of);
+        if (here != 0) {
+            const int l = __builtin_ctzll(here);
+            s.b = b0 + l;
+            s.ns = __builtin_amdgcn_readlane(c.ns, l);
+            s.piece = __builtin_amdgcn_readlane(c.piece, l);
+            s.ctx = __builtin_amdgcn_readlane(ctx, l);
+            s.first = before + __builtin_amdgcn_readlane(sum, l) - s.ns;
+            s.split = slot - s.first;
+            return s;
+        }
+        before += __builtin_amdgcn_readlane(sum, kWave - 1);
+    }
+    return s;
+}
+
+// Maximum and sum of one query row over its ns splits by 16 lanes, of which this
+// is j; every lane gets them.  Splits without weight (l = 0) count nothing; a row
+// without any has l = 0.
+__device__ __forceinline__ void merge_stats(const float* mp, const float* lp, int ns, int j, float& m, float& l) {
     float M = kLowest, L = 0.f;
-    for (int s = lane; s < ns; s += kWave) {
-        const float ls = coherent_load(lp + s), ms = ls == 0.f ? kLowest : coherent_load(mp + s);
-        const float mn = fmaxf(M, ms);
-        L = L * exp2_fast(M - mn) + ls * exp2_fast(ms - mn);
+    for (int s = j; s < ns; s += 16) {
+        const float ls = coherent_load(lp + s), ms = coherent_load(mp + s);
+        const float mn = ls == 0.f ? M : fmaxf(M, ms);
+        L = L * exp2_fast(M - mn) + (ls == 0.f ? 0.f : ls * exp2_fast(ms - mn));
         M = mn;
     }
-    m = wave_max(M);
-    l = wave_sum(L * exp2_fast(M - m));
+    m = M;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
+    l = L * exp2_fast(M - m);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) l += __shfl_xor(l, d, kWave);
 }
 
-// Head `head`'s output row from its ns split partials, by `threads` threads of
-// which this is tid: 4 channels each and every SG-th split, joined through LDS.
+// Output rows head0, head0 + step, ... (count of them) of a sequence and kv head
+// from their ns split partials, whose first is partial `first` of row `prow` on;
+// row_m and row_l: their maxima and sums.  A thread has 4 channels of a row and
+// every SG-th split.
 template <int D, class T>
-__device__ __forceinline__ void merge_row(const Params& a, size_t row, int ns, float m, float l, int tid) {
-    constexpr int UNITS = D / 4, SG = kThreads / UNITS;
-    __shared__ f32x4 part[kThreads];
-    const int u = tid % UNITS, sg = tid / UNITS;
-    const float* mp = a.m_part + row * a.num_splits;
-    const float* lp = a.l_part + row * a.num_splits;
-    const float* op = a.o_part + (row * a.num_splits) * D + u * 4;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = sg; s < ns; s += SG) {
-        const float ls = coherent_load(lp + s);
-        if (ls == 0.f) continue;
-        const float w = ls * exp2_fast(coherent_load(mp + s) - m) * inv;
+__device__ __forceinline__ void merge_rows(const Params& a, size_t row0, size_t prow0, int first, int ns, int head0,
+                                           int step, int count, const float* row_m, const float* row_l, f32x4* part,
+                                           int tid) {
+    constexpr int UNITS = D / 4, ROWS = kThreads / UNITS;
+    int rows = 1;  // at a time: a power of two
+    while (rows < ROWS && rows < count) rows *= 2;
+    const int SG = ROWS / rows, u = tid % UNITS, r = tid / UNITS % rows, sg = tid / UNITS / rows;
+    for (int k0 = 0; k0 < count; k0 += rows) {
+        const int k = k0 + r, h = head0 + k * step;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        if (k < count && row_l[h] != 0.f) {
+            const size_t at = (prow0 + h) * a.slots + first;
+            const float m = row_m[h], inv = 1.f / row_l[h];
+            for (int s0 = sg; s0 < ns; s0 += 4 * SG) {
+                float ms[4], ls[4];
+                f32x4 os[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += w * coherent_load(op + (size_t)s * D + i);
-    }
-    __syncthreads();  // a row before this one may still be read
-    part[tid] = o;
-    __syncthreads();
-    if (sg == 0) {
+                for (int i = 0; i < 4; ++i) {  // the loads of four splits together
+                    const size_t from = at + min(s0 + i * SG, ns - 1);
+                    ls[i] = s0 + i * SG < ns ? coherent_load(a.l_part + from) : 0.f;
+                    ms[i] = coherent_load(a.m_part + from);
+                    os[i] = coherent_load4(a.o_part + from * D + u * 4);
+                }
 #pragma unroll
-        for (int k = 1; k < SG; ++k) o += part[k * UNITS + u];
-        uint32_t* dst = static_cast<uint32_t*>(a.out) + (row * D + u * 4) / 2;
-        dst[0] = Half<T>::pack(o[0], o[1]);
-        dst[1] = Half<T>::pack(o[2], o[3]);
+                for (int i = 0; i < 4; ++i)
+                    if (ls[i] != 0.f) {
+                        const float w = ls[i] * exp2_fast(ms[i] - m) * inv;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] += w * os[i][e];
+                    }
+            }
+        }
+        if (SG > 1) {
+            __syncthreads();  // the rows before may still be read
+            part[tid] = o;
+            __syncthreads();
+            if (sg == 0)
+                for (int i = 1; i < SG; ++i) o += part[tid + i * UNITS * rows];
+        }
+        if (sg == 0 && k < count) {
+            uint32_t* dst = static_cast<uint32_t*>(a.out) + ((row0 + h) * D + u * 4) / 2;
+            dst[0] = Half<T>::pack(o[0], o[1]);
+            dst[1] = Half<T>::pack(o[2], o[3]);
+        }
     }
 }
 
@@ -138,17 +229,17 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     __shared__ float red_m[kWaves][kMaxGroup], red_l[kWaves][kMaxGroup];
     __shared__ int last;
 
-    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
+    const int kvh = blockIdx.x % a.hkv;
     const int G = a.group, hq = a.hkv * G;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int ctx = min(a.ctx_lens[b], a.max_tok);
-    const int start = split * a.partition, end = min(ctx, start + a.partition);
+    const Segment sg = segment(a, blockIdx.x / a.hkv, 0, lane);
+    if (sg.b < 0) return;
+    const int b = sg.b, start = sg.split * sg.piece, end = min(sg.ctx, start + sg.piece);
     const size_t row0 = (size_t)b * hq + (size_t)kvh * G;
-    const int ns = ctx > 0 ? (ctx + a.partition - 1) / a.partition : 0;
-    const bool direct = !WEIGHTS && (a.num_splits == 1 || (a.counters && ns <= 1));
-    if (start >= end) {
-        if (direct && split == 0)
+    const bool direct = !WEIGHTS && sg.ns == 1;
+    if (start >= end) {  // an empty context
+        if (direct)
             for (int i = tid; i < G * D / 2; i += kThreads) static_cast<uint32_t*>(a.out)[row0 * (D / 2) + i] = 0;
         return;
     }
@@ -297,14 +388,11 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
                 *reinterpret_cast<f32x4*>(scores + tile + 16) = s[1];
             }
         }
-        float p[8];
-        bool ok = true;
+        float p[8], bias = kShift - m_own;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
-            ok = ok && p[i] <= kPMax;
-        }
-        if (__builtin_amdgcn_ballot_w64(!ok)) {
+        for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] + bias);
+        const float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+        if (__builtin_amdgcn_ballot_w64(top > kPMax)) {
             // Move the reference maximum of every head to its running maximum.
             float mx = m_own;
 #pragma unroll
@@ -320,8 +408,9 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
 #pragma unroll
                 for (int j = 0; j < DPL; ++j) acc[j][r] *= al;
             }
+            bias = kShift - m_own;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] - m_own + kShift);
+            for (int i = 0; i < 8; ++i) p[i] = exp2_fast(s[i / 4][i % 4] + bias);
         }
         l_own += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         u32x4 pf;
@@ -417,7 +506,6 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
             for (int j = 0; j < DPL; ++j) red_acc[w][4 * g + r][DPL * n + j] = acc[j][r];
         }
     __syncthreads();
-    const bool fused = !WEIGHTS && a.counters && !direct;
     for (int i = tid; i < G * D / 2; i += kThreads) {
         const int h = i / (D / 2), d = 2 * (i % (D / 2));
         float M = red_m[0][h];
@@ -432,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
             o1 += red_acc[v][h][d + 1] * wv;
         }
         const float inv = L == 0.f ? 0.f : 1.f / L;  // no token that counts: zeros
-        const size_t slot = (row0 + h) * a.num_splits + split;
+        const size_t slot = (size_t)(kvh * G + h) * a.slots + sg.first + sg.split;
         if (direct) {
             static_cast<uint32_t*>(a.out)[((row0 + h) * D + d) / 2] = Half<T>::pack(o0 * inv, o1 * inv);
         } else {
@@ -444,25 +532,26 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
             }
         }
     }
-    if (!fused) return;
+    if (WEIGHTS || direct || !a.counters) return;
     // The last split of the sequence and kv head to finish merges them all.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     int32_t* cnt = a.counters + (size_t)b * a.hkv + kvh;
-    if (tid == 0) last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
+    if (tid == 0) last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == sg.ns - 1;
     __syncthreads();
     if (!last) return;
     if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int h = w; h < G; h += kWaves) {
+    const size_t prow0 = (size_t)kvh * G;
+    if (const int h = tid / 16; h < G) {
         float m, l;
-        merge_stats(a.m_part + (row0 + h) * a.num_splits, a.l_part + (row0 + h) * a.num_splits, ns, lane, m, l);
-        if (lane == 0) {
-            red_m[0][h] = m;
-            red_l[0][h] = l;
-        }
+        const size_t at = (prow0 + h) * a.slots + sg.first;
+        merge_stats(a.m_part + at, a.l_part + at, sg.ns, tid % 16, m, l);
+        red_m[0][h] = m;
+        red_l[0][h] = l;
     }
     __syncthreads();
-    for (int h = 0; h < G; ++h) merge_row<D, T>(a, row0 + h, ns, red_m[0][h], red_l[0][h], tid);
+    merge_rows<D, T>(a, row0, prow0, sg.first, sg.ns, 0, 1, G, red_m[0], red_l[0],
+                     reinterpret_cast<f32x4*>(&red_acc[0][0][0]), tid);
 }
 
 // After decode_mx_kernel: merges the splits' outputs, and turns the scores into
@@ -471,37 +560,55 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
 template <int D, class T, bool WEIGHTS>
 __global__ void __launch_bounds__(kThreads) decode_mx_finish_kernel(const Params a) {
     __shared__ float row_m[kMaxGroup], row_l[kMaxGroup];
+    __shared__ f32x4 part[kThreads];
     const int c = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     const int G = a.group, hq = a.hkv * G;
-    const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
-    const int ctx = max(min(a.ctx_lens[b], a.max_tok), 0);
-    const size_t row0 = (size_t)b * hq + (size_t)kvh * G;
-    const int ns = (ctx + a.partition - 1) / a.partition;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int ctx = context(a, b);
     const int active = WEIGHTS ? max((ctx + kFinishTokens - 1) / kFinishTokens, 1) : gridDim.x;
     if (c >= active) return;
-    for (int h = w; h < G; h += kWaves) {
+    const size_t row0 = (size_t)b * hq + (size_t)kvh * G, prow0 = (size_t)kvh * G;
+    // The first heads' scores are on their way while the splits are merged.
+    constexpr int HEADS = 8;
+    const int t = c * kFinishTokens + 2 * tid;
+    const float* scores = a.scores + row0 * a.scores_stride + t;
+    f32x2 s[HEADS];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i)
+            if (h0 + i < G && t < ctx)
+                s[i] = *reinterpret_cast<const f32x2*>(scores + (size_t)(h0 + i) * a.scores_stride);
+    };
+    if constexpr (WEIGHTS) load(0);
+    const Segment sg = segment(a, -1, b, lane);
+    if (!WEIGHTS && sg.ns == 1) return;  // written by decode_mx_kernel
+    if (const int h = tid / 16; h < G) {
         float m, l;
-        merge_stats(a.m_part + (row0 + h) * a.num_splits, a.l_part + (row0 + h) * a.num_splits, ns, lane, m, l);
-        if (lane == 0) {
-            row_m[h] = m;
-            row_l[h] = l;
-        }
+        const size_t at = (prow0 + h) * a.slots + sg.first;
+        merge_stats(a.m_part + at, a.l_part + at, ctx > 0 ? sg.ns : 0, tid % 16, m, l);
+        row_m[h] = m;
+        row_l[h] = l;
     }
     __syncthreads();
     if constexpr (WEIGHTS) {
-        float* wt = a.weights + b * a.w_stride_b + kvh * a.w_stride_h;
-        const int t0 = c * kFinishTokens, t1 = min(ctx, t0 + kFinishTokens);
-        for (int t = t0 + tid; t < t1; t += kThreads) {
-            const float* s = a.scores + row0 * a.scores_stride + t;
-            float sum = 0.f;
-            for (int h = 0; h < G; ++h) {
-                const float l = row_l[h];
-                if (l != 0.f) sum += exp2_fast(s[h * a.scores_stride] - row_m[h]) * (1.f / l);
-            }
-            wt[t] += sum;
+        float sum[2] = {0.f, 0.f};
+        for (int h0 = 0; h0 < G; h0 += HEADS) {
+            if (h0 > 0) load(h0);
+#pragma unroll
+            for (int i = 0; i < HEADS; ++i)
+                if (h0 + i < G && row_l[h0 + i] != 0.f) {
+                    const float inv = 1.f / row_l[h0 + i], m = row_m[h0 + i];
+                    sum[0] += exp2_fast(s[i][0] - m) * inv;
+                    sum[1] += exp2_fast(s[i][1] - m) * inv;
+                }
         }
+        float* wt = a.weights + b * a.w_stride_b + kvh * a.w_stride_h + t;
+        if (t < ctx) wt[0] += sum[0];
+        if (t + 1 < ctx) wt[1] += sum[1];
     }
-    for (int h = c; h < G; h += active) merge_row<D, T>(a, row0 + h, ns, row_m[h], row_l[h], tid);
+    if (c < G)
+        merge_rows<D, T>(a, row0, prow0, sg.first, ctx > 0 ? sg.ns : 0, c, active, (G - c + active - 1) / active, row_m,
+                         row_l, part, tid);
 }
 
 template <int D, class T, bool MX, bool WEIGHTS>
@@ -530,14 +637,14 @@ hipError_t launch(const DecodeMxArgs& x) {
     p.max_blocks = (int)x.max_blocks;
     p.num_blocks = (int)x.num_blocks;
     p.max_tok = (int)std::min(x.max_blocks * x.bs, x.max_ctx);
+    p.batch = (int)x.batch;
     p.partition = (int)x.partition;
-    p.num_splits = (int)x.num_splits;
+    p.slots = (int)x.slots;
     p.sl2 = x.sl2;
-    const bool merge_here = !WEIGHTS && x.num_splits <= kFusedMaxSplits;
-    p.counters = merge_here ? x.counters : nullptr;
-    const dim3 grid((unsigned)x.hkv, (unsigned)x.num_splits, (unsigned)x.batch);
-    hipLaunchKernelGGL((decode_mx_kernel<D, T, MX, WEIGHTS>), grid, dim3(kThreads), 0, (hipStream_t)x.stream, p);
-    if (merge_here && (x.num_splits == 1 || x.counters)) return hipGetLastError();
+    p.counters = WEIGHTS ? nullptr : x.counters;
+    hipLaunchKernelGGL((decode_mx_kernel<D, T, MX, WEIGHTS>), dim3((unsigned)(x.hkv * x.slots)), dim3(kThreads), 0,
+                       (hipStream_t)x.stream, p);
+    if (!WEIGHTS && (x.slots == x.batch || x.counters)) return hipGetLastError();
     const unsigned chunks = WEIGHTS ? (unsigned)((p.max_tok + kFinishTokens - 1) / kFinishTokens) : (unsigned)p.group;
     hipLaunchKernelGGL((decode_mx_finish_kernel<D, T, WEIGHTS>), dim3(chunks, (unsigned)x.hkv, (unsigned)x.batch),
                        dim3(kThreads), 0, (hipStream_t)x.stream, p);
@@ -552,12 +659,15 @@ hipError_t launch_typed(const DecodeMxArgs& x) {
 
 }  // namespace
 
-// About four workgroups for each of the 256 CUs.
-int64_t decode_mx_partition(int64_t batch, int64_t hkv, int64_t max_ctx) {
-    constexpr int64_t kChunk = 256, kWorkgroups = 1024;
-    const int64_t chunks = (max_ctx + kChunk - 1) / kChunk;
-    const int64_t splits = std::min(chunks, (kWorkgroups + batch * hkv - 1) / (batch * hkv));
-    return (chunks + splits - 1) / splits * kChunk;
+// Splits of a kv head over the whole batch.  Cut evenly: as many as fit the 256
+// CUs at once (four workgroups each), at least two a sequence on average, none
+// of less than kMinSplit tokens, and no more than 64 a sequence for one workgroup
+// to merge.
+int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition) {
+    if (partition > 0) return batch * ((max_ctx + partition - 1) / partition);
+    constexpr int64_t kWorkgroups = 1024, kMostSplits = 64;
+    const int64_t chunks = std::min(kMostSplits, (max_ctx + kMinSplit - 1) / kMinSplit);
+    return std::min(batch * chunks, std::max((kWorkgroups + hkv - 1) / hkv, 2 * batch));
 }
 
 hipError_t decode_mx_launch(const DecodeMxArgs& x) {

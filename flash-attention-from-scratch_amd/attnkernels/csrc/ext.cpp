@@ -514,9 +514,10 @@ static torch::Tensor decode_mx(const torch::Tensor& q, const torch::Tensor& kc, 
     const at::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     const torch::Tensor q1 = aligned(q), bt = int_array(block_tables), ctx = int_array(context_lens);
     auto out = torch::empty({B, hq, D}, q.options());
-    const int64_t partition = partition_size.has_value() ? (*partition_size + 255) / 256 * 256
-                                                         : ak_paged_decode_mx_partition(B, hkv, max_ctx);
-    const size_t ws_bytes = ak_paged_decode_mx_workspace_size(B, hq, D, max_ctx, partition, weights != nullptr);
+    require(!partition_size.has_value() || (*partition_size >= 1 && *partition_size <= INT32_MAX / 2),
+            "partition_size must be at least 1");
+    const int64_t partition = partition_size.has_value() ? (*partition_size + 255) / 256 * 256 : 0;
+    const size_t ws_bytes = ak_paged_decode_mx_workspace_size(B, hq, hkv, D, max_ctx, partition, weights != nullptr);
     torch::Tensor ws, counters;
     if (ws_bytes > 0) ws = torch::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
     if (ws_bytes > 0 && !weights) counters = split_counters(q, B * hkv);

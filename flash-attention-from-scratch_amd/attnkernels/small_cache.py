@@ -56,8 +56,8 @@ def paged_decode_mxfp4(q, k_cache, k_scales, v_cache, v_scales, block_tables, co
     block_tables, context_lens, max_context_len, scale: as in paged_decode; a
                   context of 0 tokens gives zeros, tokens from max_context_len on
                   are ignored
-    partition_size: tokens per split (rounded up to a multiple of 256); None: about
-                  four workgroups per CU
+    partition_size: tokens per split (rounded up to a multiple of 256); None: the
+                  kernel cuts the contexts into splits of about equal size
     weights:      None, or float32 [B, H_kv, >= max_context_len], to which each
                   token's softmax weight is added, summed over the query heads of its
                   kv head (``paged_decode_weights``)

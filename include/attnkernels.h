@@ -246,19 +246,19 @@ int ak_gather_cache_mxfp4(const void *k_cache, const void *k_scales, const void 
                           int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
                           int64_t num_blocks, int64_t block_size, int bf16, void *stream);
 
-/* Tokens per split that suit these sizes (a multiple of 256), and the workspace
- * of the two calls below: with_weights != 0 where weights are given. 0 bytes:
- * none is needed; 0 too for invalid sizes. */
-int64_t ak_paged_decode_mx_partition(int64_t batch, int64_t num_kv_heads, int64_t max_context_len);
-size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64_t head_dim,
-                                         int64_t max_context_len, int64_t partition, int with_weights);
+/* Workspace of the two calls below, with_weights != 0 where weights are given; 0:
+ * none is needed (or invalid sizes). */
+size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                                         int64_t head_dim, int64_t max_context_len, int64_t partition,
+                                         int with_weights);
 
 /* Paged decode over MXFP4 caches, num_heads / num_kv_heads from 1 to 16, and,
  * where weights is not NULL, weights[b, kv head, t] += sum over the kv head's
  * query heads of token t's softmax weight.  Tokens at or past
- * max_context_len are ignored; weights_length >= max_context_len.  Arguments
- * otherwise as in ak_paged_decode_fused (counters may be NULL; they are not used
- * with weights). */
+ * max_context_len are ignored; weights_length >= max_context_len.  partition: tokens
+ * per split, a multiple of 256; 0: the kernel cuts the splits evenly from the
+ * context lengths.  Arguments otherwise as in ak_paged_decode_fused (counters may be
+ * NULL; they are not used with weights). */
 int ak_paged_decode_mxfp4(const void *q, const void *k_cache, const void *k_scales, const void *v_cache,
                           const void *v_scales, const int32_t *block_tables, const int32_t *context_lens,
                           void *out, float *weights, int64_t weights_stride_b, int64_t weights_stride_h,

@@ -209,9 +209,7 @@ def lib():
     L.ak_last_error.restype = ctypes.c_char_p
     L.ak_reshape_and_cache_mxfp4.argtypes = [vp] * 7 + [i64] * 7 + [ci, vp]
     L.ak_gather_cache_mxfp4.argtypes = [vp] * 7 + [i64] * 5 + [ci, vp]
-    L.ak_paged_decode_mx_partition.argtypes = [i64] * 3
-    L.ak_paged_decode_mx_partition.restype = i64
-    L.ak_paged_decode_mx_workspace_size.argtypes = [i64] * 5 + [ci]
+    L.ak_paged_decode_mx_workspace_size.argtypes = [i64] * 6 + [ci]
     L.ak_paged_decode_mx_workspace_size.restype = sz
     L.ak_paged_decode_mxfp4.argtypes = [vp] * 9 + [i64] * 11 + [f64, i64, ci, vp, sz, vp, i64, vp]
     L.ak_paged_decode_weights.argtypes = [vp] * 7 + [i64] * 11 + [f64, i64, ci, vp, sz, vp]
@@ -256,7 +254,7 @@ def _decode(lib, weights=FAKE, full=False, **over):
 
 
 @pytest.mark.parametrize("code,word,over", [
-    (1, "multiple of num_kv_heads", dict(hq=5)), (1, "positive multiple of 256", dict(part=100)),
+    (1, "multiple of num_kv_heads", dict(hq=5)), (1, "positive multiple of 256", dict(part=100)), (1, "positive multiple of 256", dict(part=-256)),
     (2, "at most 16", dict(hq=34)), (2, "head_dim", dict(d=32)), (1, "invalid size", dict(bs=0)),
     (1, "max_context_len", dict(ctx=0)), (1, "empty block table", dict(mb=0)), (1, "null", dict(q=None)),
     (1, "aligned", dict(q=FAKE + 2)), (1, "out of range", dict(ctx=1 << 31, wl=1 << 31, wh=1 << 31, wb=1 << 32)),
@@ -274,18 +272,12 @@ def test_capi_decode_more_refusals(lib):
     _refused(lib, _decode(lib, weights=None, full=True), 1, "null")
     _refused(lib, _decode(lib, weights=None, counters=FAKE, ncount=3), 1, "counters")
     _refused(lib, _decode(lib, weights=None, ctx=1000, bytes=64), 3, "bytes required")
-    _refused(lib, _decode(lib, weights=None, ctx=1 << 28, part=256, bytes=1 << 62), 1, "splits")
+    _refused(lib, _decode(lib, weights=None, ctx=1 << 29, part=256, bytes=1 << 62, batch=2000), 1, "splits")
     assert _decode(lib, batch=0) == 0
-    assert lib.ak_paged_decode_mx_workspace_size(2, 4, 64, 40, 256, 0) == 0
-    assert lib.ak_paged_decode_mx_workspace_size(2, 4, 64, 40, 256, 1) >= 2 * 4 * (66 + 64) * 4
-
-
-def test_partition_is_a_multiple_of_256_that_covers(lib):
-    for batch in (1, 3, 16, 64, 1000):
-        for hkv in (1, 8, 32):
-            for ctx in (1, 255, 256, 257, 4096, 100000, 1 << 24):
-                p = lib.ak_paged_decode_mx_partition(batch, hkv, ctx)
-                assert p > 0 and p % 256 == 0 and -(-ctx // p) <= 65535
+    for part in (0, 256):
+        assert lib.ak_paged_decode_mx_workspace_size(2, 4, 2, 64, 40, part, 0) == 0
+        assert lib.ak_paged_decode_mx_workspace_size(2, 4, 2, 64, 40, part, 1) >= 2 * 4 * (66 + 64) * 4
+    assert lib.ak_paged_decode_mx_workspace_size(2, 4, 2, 64, 1000, 0, 0) > 0
 
 
 def _prompt(lib, **over):
