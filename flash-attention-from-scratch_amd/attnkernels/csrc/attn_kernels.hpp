@@ -102,6 +102,7 @@ struct DecodeMxArgs {
     float* o_part;         // [hq, slots, D]  split partials
     float* m_part;         // [hq, slots]
     float* l_part;         // [hq, slots]
+    void* cuts;            // [batch] pairs of int32
     float* scores;         // [B, hq, scores_stride]: scale * log2(e) * q.k, where weights are wanted
     float* weights;        // [B, hkv, >= max_ctx], strides in elements below
     int32_t* counters;     // one per (sequence, kv head), zero on entry and left zero

@@ -280,9 +280,11 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
         a.o_part = static_cast<float*>(workspace);
         a.m_part = a.o_part + rows * (size_t)head_dim;
         a.l_part = a.m_part + rows;
+        size_t at = (partials_bytes(1, num_heads, slots, head_dim) + 7) / 8 * 8;
+        a.cuts = static_cast<char*>(workspace) + at;
         if (weights) {
-            a.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                                round16(partials_bytes(1, num_heads, slots, head_dim)));
+            at = round16(at + (size_t)batch * 2 * sizeof(int32_t));
+            a.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + at);
             a.scores_stride = scores_row(max_context_len);
         }
     }
@@ -563,7 +565,7 @@ size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64
         return 0;
     const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition);
     if (slots <= batch && !with_weights) return 0;
-    const size_t parts = partials_bytes(1, num_heads, slots, head_dim);
+    const size_t parts = partials_bytes(1, num_heads, slots, head_dim) + (size_t)batch * 2 * sizeof(int32_t) + 8;
     return with_weights ? round16(parts) + (size_t)batch * (size_t)num_heads * (size_t)scores_row(max_context_len) *
                                                sizeof(float)
                         : parts;

@@ -41,7 +41,6 @@ namespace {
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kTile = 32;           // tokens per wave iteration
 constexpr int kMaxGroup = 16;       // query heads per kv head: rows of the MFMA
-constexpr int kFinishTokens = 512;  // tokens per workgroup of the finishing kernel: two of a thread
 constexpr int kCut = kWaves * kTile; // splits start at multiples of it
 constexpr int kMinSplit = 256;
 constexpr float kLowest = -3.402823466e38f;
@@ -53,6 +52,7 @@ struct Params {
     void* out;
     float *o_part, *m_part, *l_part, *scores, *weights;
     int32_t* counters;
+    int2* cuts;            // [batch]: a sequence's first slot and its splits, for the finishing kernel
     int64_t scores_stride, w_stride_b, w_stride_h;
     int batch, hkv, group, bs, bs_shift, max_blocks, num_blocks, max_tok;
     int partition;  // tokens per split; 0: cut evenly
@@ -91,8 +91,17 @@ __device__ __forceinline__ Cut cut_context(int len, int size) {
 
 __device__ __forceinline__ int context(const Params& a, int b) { return max(min(a.ctx_lens[b], a.max_tok), 0); }
 
-// Tokens per split.  Cut evenly: so many that the splits of all sequences fit the
-// slots: sum ceil(len / size) <= sum len / size + batch.
+__device__ __forceinline__ int wave_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8: a row's last lane has its sum
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    return __builtin_amdgcn_readlane(x, 15) + __builtin_amdgcn_readlane(x, 31) + __builtin_amdgcn_readlane(x, 47) +
+           __builtin_amdgcn_readlane(x, 63);
+}
+
+// Tokens per split.  Cut evenly: the smallest of five sizes whose splits fit the
+// slots; the last one always does: sum ceil(len / size) <= sum len / size + batch.
 __device__ __forceinline__ int split_size(const Params& a, int lane) {
     if (a.partition > 0) return a.partition;
     if (a.slots <= a.batch) return INT32_MAX / 4 / kCut * kCut;  // a split each
@@ -100,16 +109,23 @@ __device__ __forceinline__ int split_size(const Params& a, int lane) {
     for (int b = lane; b < a.batch; b += kWave) total += (float)context(a, b);
 #pragma unroll
     for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
-    const float size = total * 1.0005f / (float)(a.slots - a.batch) + 1.f;
-    return max(((int)size + kCut) / kCut * kCut, kMinSplit);
+    for (int spare = 0;; ++spare) {
+        const float of = (float)a.slots - (float)a.batch * 0.25f * (float)spare;
+        const int size = max((int)(total * (spare < 4 ? 1.f : 1.0005f) / of + kCut) / kCut * kCut, kMinSplit);
+        if (spare == 4) return size;
+        int count = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += kWave)
+            count += wave_sum(b0 + lane < a.batch ? cut_context(context(a, b0 + lane), size).ns : 0);
+        if (count <= a.slots) return size;
+    }
 }
 
-// The split that slot `slot` holds, or slot 0 of sequence `of` (slot < 0): every
-// wave counts the splits of the sequences in order.  b < 0: none.
+// The split that slot `slot` holds: every wave counts the splits of the sequences
+// in order.  b < 0: none.
 struct Segment {
     int b, split, ns, piece, first, ctx;  // first: the sequence's first slot
 };
-__device__ __forceinline__ Segment segment(const Params& a, int slot, int of, int lane) {
+__device__ __forceinline__ Segment segment(const Params& a, int slot, int lane) {
     Segment s;
     s.b = -1;
     const int size = split_size(a, lane);
@@ -123,7 +139,7 @@ __device__ __forceinline__ Segment segment(const Params& a, int slot, int of, in
             const int y = __shfl_up(sum, d, kWave);
             if (lane >= d) sum += y;
         }
-        const uint64_t here = __builtin_amdgcn_ballot_w64(slot >= 0 ? before + sum > slot : b == of);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(before + sum > slot);
         if (here != 0) {
             const int l = __builtin_ctzll(here);
             s.b = b0 + l;
@@ -210,12 +226,25 @@ __device__ __forceinline__ void merge_rows(const Params& a, size_t row0, size_t 
     }
 }
 
+// A register with x in its low bits and anything above.
+__device__ __forceinline__ uint32_t loose(uint32_t x) { return x; }
+__device__ __forceinline__ uint32_t loose(uint16_t x) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 y;
+    y[0] = x;
+    return __builtin_bit_cast(uint32_t, y);
+}
+
 template <int D, class T, bool MX>
 struct Tile {
     static constexpr int KW = MX ? D / 32 : D / 8;    // dwords of K per block: a quarter row
     static constexpr int VW = MX ? 1 : D / 32;        // dwords of a V row's D/16 channels (4 bits, D = 64: half of one)
-    uint32_t k[2][KW], v[2][4][VW];
-    uint32_t ks[2], vs[2][4];
+    // The two-byte words of D = 64 stay two bytes until they are used: widened
+    // where they are loaded, the compiler would wait for them there.
+    typedef std::conditional_t<MX && D == 64, uint16_t, uint32_t> word_t;
+    uint32_t k[2][KW];
+    word_t v[2][4][VW];
+    word_t ks[2], vs[2][4];  // a row's scales: 4 or 2 bytes
 };
 
 template <int D, class T, bool MX, bool WEIGHTS>
@@ -233,11 +262,12 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     const int G = a.group, hq = a.hkv * G;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const Segment sg = segment(a, blockIdx.x / a.hkv, 0, lane);
+    const Segment sg = segment(a, blockIdx.x / a.hkv, lane);
     if (sg.b < 0) return;
     const int b = sg.b, start = sg.split * sg.piece, end = min(sg.ctx, start + sg.piece);
     const size_t row0 = (size_t)b * hq + (size_t)kvh * G;
     const bool direct = !WEIGHTS && sg.ns == 1;
+    if (a.cuts && sg.split == 0 && kvh == 0 && tid == 0) a.cuts[b] = int2{sg.first, sg.ns};
     if (start >= end) {  // an empty context
         if (direct)
             for (int i = tid; i < G * D / 2; i += kThreads) static_cast<uint32_t*>(a.out)[row0 * (D / 2) + i] = 0;
@@ -261,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     // What a lane loads of a block's rows: byte offsets from the block's first
     // row.  Of the scales it loads a row's (4 or 2 bytes) and shifts its group's.
     constexpr int SROW = D / 32;
-    typedef std::conditional_t<D == 128, uint32_t, uint16_t> scales_t;
+    typedef typename Tl::word_t word_t;
     const uint32_t k_off = n * KROW + (MX ? KROW / 4 : 16) * g, v_off = 4 * g * KROW + KROW / 16 * n;
     const uint32_t k_shift = g / (4 / SROW) * 8, v_shift = n / (16 / SROW) * 8;
     auto load_k = [&](Tl& x, int blk, const char* p, const uint8_t* sc) {
@@ -282,22 +312,22 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
                 for (int i = 0; i < 4; ++i) x.k[blk][4 * s + i] = y[i];
             }
         }
-        if constexpr (MX) x.ks[blk] = *reinterpret_cast<const scales_t*>(sc);
+        if constexpr (MX) x.ks[blk] = *reinterpret_cast<const word_t*>(sc);
     };
     auto load_v = [&](Tl& x, int blk, int r, const char* p, const uint8_t* sc) {
         if constexpr (MX && D == 128) {
             x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
         } else if constexpr (MX) {
-            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p));
+            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const word_t*>(p));
         } else {
             typedef uint32_t vec __attribute__((ext_vector_type(Tl::VW)));
             const vec y = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p));
 #pragma unroll
             for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = y[i];
         }
-        if constexpr (MX) x.vs[blk][r] = *reinterpret_cast<const scales_t*>(sc);
+        if constexpr (MX) x.vs[blk][r] = *reinterpret_cast<const word_t*>(sc);
     };
-    auto group_scale = [](uint32_t word, uint32_t shift) { return mx_scale(word >> shift & 255u); };
+    auto group_scale = [](word_t word, uint32_t shift) { return mx_scale(loose(word) >> shift & 255u); };
     // A tile each of whose two blocks is in one page: K's or V's loads at scalar
     // bases, pa and pb the pages.
     auto load_whole = [&](Tl& x, int tile, int pa, int pb, auto what) {
@@ -433,10 +463,10 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
 #pragma unroll
             for (int i = 0; i < 8; ++i) sc[i] = group_scale(x.vs[i / 4][i % 4], v_shift);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<0>(x.v[i / 4][i % 4][0], sc[i]);
+            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<0>(loose(x.v[i / 4][i % 4][0]), sc[i]);
             channels(v, 0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<1>(x.v[i / 4][i % 4][0], sc[i]);
+            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<1>(loose(x.v[i / 4][i % 4][0]), sc[i]);
             channels(v, 1);
             if constexpr (DPL == 8) {
 #pragma unroll
@@ -555,60 +585,69 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
 }
 
 // After decode_mx_kernel: merges the splits' outputs, and turns the scores into
-// weights.  Workgroup c of a (kv head, sequence) has tokens c * kFinishTokens on
-// and the heads h with h % (workgroups with tokens) == c.
-template <int D, class T, bool WEIGHTS>
+// weights, TOKENS of a thread (0: no weights).  Workgroup c of a (kv head,
+// sequence) has its tokens from c * kThreads * TOKENS on and the heads h with
+// h % (workgroups with tokens) == c.
+template <int D, class T, int TOKENS>
 __global__ void __launch_bounds__(kThreads) decode_mx_finish_kernel(const Params a) {
+    constexpr int N = TOKENS > 0 ? TOKENS : 1;
+    typedef float scores_t __attribute__((ext_vector_type(N)));
     __shared__ float row_m[kMaxGroup], row_l[kMaxGroup];
     __shared__ f32x4 part[kThreads];
     const int c = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     const int G = a.group, hq = a.hkv * G;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int ctx = context(a, b);
-    const int active = WEIGHTS ? max((ctx + kFinishTokens - 1) / kFinishTokens, 1) : gridDim.x;
+    const int active = TOKENS > 0 ? max((ctx + kThreads * N - 1) / (kThreads * N), 1) : gridDim.x;
     if (c >= active) return;
+    const int2 cut = a.cuts[b];
+    const int first = cut.x, ns = ctx > 0 ? cut.y : 0;
+    if (TOKENS == 0 && cut.y == 1) return;  // written by decode_mx_kernel
     const size_t row0 = (size_t)b * hq + (size_t)kvh * G, prow0 = (size_t)kvh * G;
     // The first heads' scores are on their way while the splits are merged.
     constexpr int HEADS = 8;
-    const int t = c * kFinishTokens + 2 * tid;
-    const float* scores = a.scores + row0 * a.scores_stride + t;
-    f32x2 s[HEADS];
+    const int t = (c * kThreads + tid) * N;
+    scores_t s[HEADS];
     auto load = [&](int h0) {
+        const float* scores = a.scores + row0 * a.scores_stride + t;
 #pragma unroll
         for (int i = 0; i < HEADS; ++i)
             if (h0 + i < G && t < ctx)
-                s[i] = *reinterpret_cast<const f32x2*>(scores + (size_t)(h0 + i) * a.scores_stride);
+                s[i] = *reinterpret_cast<const scores_t*>(scores + (size_t)(h0 + i) * a.scores_stride);
     };
-    if constexpr (WEIGHTS) load(0);
-    const Segment sg = segment(a, -1, b, lane);
-    if (!WEIGHTS && sg.ns == 1) return;  // written by decode_mx_kernel
+    float* wt = a.weights + b * a.w_stride_b + kvh * a.w_stride_h + t;
+    float old[N];
+    if constexpr (TOKENS > 0) {
+        load(0);
+#pragma unroll
+        for (int j = 0; j < N; ++j) old[j] = t + j < ctx ? wt[j] : 0.f;
+    }
     if (const int h = tid / 16; h < G) {
         float m, l;
-        const size_t at = (prow0 + h) * a.slots + sg.first;
-        merge_stats(a.m_part + at, a.l_part + at, ctx > 0 ? sg.ns : 0, tid % 16, m, l);
+        const size_t at = (prow0 + h) * a.slots + first;
+        merge_stats(a.m_part + at, a.l_part + at, ns, tid % 16, m, l);
         row_m[h] = m;
         row_l[h] = l;
     }
     __syncthreads();
-    if constexpr (WEIGHTS) {
-        float sum[2] = {0.f, 0.f};
+    if constexpr (TOKENS > 0) {
+        float sum[N] = {};
         for (int h0 = 0; h0 < G; h0 += HEADS) {
             if (h0 > 0) load(h0);
 #pragma unroll
             for (int i = 0; i < HEADS; ++i)
                 if (h0 + i < G && row_l[h0 + i] != 0.f) {
                     const float inv = 1.f / row_l[h0 + i], m = row_m[h0 + i];
-                    sum[0] += exp2_fast(s[i][0] - m) * inv;
-                    sum[1] += exp2_fast(s[i][1] - m) * inv;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) sum[j] += exp2_fast(s[i][j] - m) * inv;
                 }
         }
-        float* wt = a.weights + b * a.w_stride_b + kvh * a.w_stride_h + t;
-        if (t < ctx) wt[0] += sum[0];
-        if (t + 1 < ctx) wt[1] += sum[1];
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (t + j < ctx) wt[j] = old[j] + sum[j];
     }
     if (c < G)
-        merge_rows<D, T>(a, row0, prow0, sg.first, ctx > 0 ? sg.ns : 0, c, active, (G - c + active - 1) / active, row_m,
-                         row_l, part, tid);
+        merge_rows<D, T>(a, row0, prow0, first, ns, c, active, (G - c + active - 1) / active, row_m, row_l, part, tid);
 }
 
 template <int D, class T, bool MX, bool WEIGHTS>
@@ -642,12 +681,23 @@ hipError_t launch(const DecodeMxArgs& x) {
     p.slots = (int)x.slots;
     p.sl2 = x.sl2;
     p.counters = WEIGHTS ? nullptr : x.counters;
+    const bool finish = WEIGHTS || (x.slots > x.batch && !x.counters);
+    p.cuts = finish ? static_cast<int2*>(x.cuts) : nullptr;
     hipLaunchKernelGGL((decode_mx_kernel<D, T, MX, WEIGHTS>), dim3((unsigned)(x.hkv * x.slots)), dim3(kThreads), 0,
                        (hipStream_t)x.stream, p);
-    if (!WEIGHTS && (x.slots == x.batch || x.counters)) return hipGetLastError();
-    const unsigned chunks = WEIGHTS ? (unsigned)((p.max_tok + kFinishTokens - 1) / kFinishTokens) : (unsigned)p.group;
-    hipLaunchKernelGGL((decode_mx_finish_kernel<D, T, WEIGHTS>), dim3(chunks, (unsigned)x.hkv, (unsigned)x.batch),
-                       dim3(kThreads), 0, (hipStream_t)x.stream, p);
+    if (!finish) return hipGetLastError();
+    auto run = [&](auto* kernel, int64_t workgroups) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)workgroups, (unsigned)x.hkv, (unsigned)x.batch), dim3(kThreads), 0,
+                           (hipStream_t)x.stream, p);
+    };
+    if constexpr (WEIGHTS) {
+        // Four tokens of a thread where that leaves eight workgroups a CU.
+        const int64_t wide = (p.max_tok + 4 * kThreads - 1) / (4 * kThreads);
+        if (wide * x.hkv * x.batch >= 2048) run(decode_mx_finish_kernel<D, T, 4>, wide);
+        else run(decode_mx_finish_kernel<D, T, 2>, (p.max_tok + 2 * kThreads - 1) / (2 * kThreads));
+    } else {
+        run(decode_mx_finish_kernel<D, T, 0>, p.group);
+    }
     return hipGetLastError();
 }
 
