@@ -155,8 +155,8 @@ ak::BalancedPlan balanced_plan(int64_t batch, int64_t num_heads, int64_t num_kv_
 
 size_t round16(size_t x) { return (x + 15) / 16 * 16; }
 
-// A row of scores of ak_paged_decode_mx_*: whole tiles of 32 tokens.
-int64_t scores_row(int64_t max_context_len) { return (max_context_len + 31) / 32 * 32; }
+// A row of scores of ak_paged_decode_mx_*: whole tiles of 64 tokens.
+int64_t scores_row(int64_t max_context_len) { return (max_context_len + 63) / 64 * 64; }
 
 // Whether a [batch, kv heads, length] array of these strides has no two rows in one place.
 int weights_rows(const char* who, int64_t batch, int64_t kv_heads, int64_t stride_b, int64_t stride_h, int64_t length) {
@@ -233,7 +233,8 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
     if (max_context_len > INT_MAX / 2 || partition > INT_MAX / 2 || num_blocks > INT_MAX ||
         max_blocks_per_seq > INT_MAX / 2 / block_size || batch > 65535 || num_kv_heads > 65535)
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": size out of range");
-    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition);
+    const int64_t slots =
+        ak::decode_mx_slots(batch, num_kv_heads, head_dim, max_context_len, partition, k_scales != nullptr);
     if (slots > INT_MAX / num_kv_heads) return fail(AK_ERR_INVALID_ARGUMENT, who + ": too many splits");
     if (weights) {
         if (w_length < max_context_len)
@@ -563,7 +564,8 @@ size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64
     if (batch < 1 || num_heads < 1 || num_kv_heads < 1 || head_dim <= 0 || max_context_len < 1 || partition < 0 ||
         max_context_len > INT_MAX / 2)
         return 0;
-    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition);
+    // 4-bit caches are cut into as many splits as others, or more.
+    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, head_dim, max_context_len, partition, true);
     if (slots <= batch && !with_weights) return 0;
     const size_t parts = partials_bytes(1, num_heads, slots, head_dim) + (size_t)batch * 2 * sizeof(int32_t) + 8;
     return with_weights ? round16(parts) + (size_t)batch * (size_t)num_heads * (size_t)scores_row(max_context_len) *

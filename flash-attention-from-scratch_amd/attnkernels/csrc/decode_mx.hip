@@ -105,14 +105,13 @@ __device__ __forceinline__ int wave_sum(int x) {
 __device__ __forceinline__ int split_size(const Params& a, int lane) {
     if (a.partition > 0) return a.partition;
     if (a.slots <= a.batch) return INT32_MAX / 4 / kCut * kCut;  // a split each
-    float total = 0.f;  // off by up to a few thousand units in the last place, which the factor below covers
-    for (int b = lane; b < a.batch; b += kWave) total += (float)context(a, b);
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
+    float total = 0.f;  // in units of 64 tokens, rounded up, so that 64 of them fit an integer
+    for (int b0 = 0; b0 < a.batch; b0 += kWave)
+        total += (float)wave_sum(b0 + lane < a.batch ? (context(a, b0 + lane) + 63) / 64 : 0) * 64.f;
     for (int spare = 0;; ++spare) {
-        const float of = (float)a.slots - (float)a.batch * 0.25f * (float)spare;
-        const int size = max((int)(total * (spare < 4 ? 1.f : 1.0005f) / of + kCut) / kCut * kCut, kMinSplit);
-        if (spare == 4) return size;
+        const float of = fmaxf((float)a.slots - (float)a.batch * 0.25f * (float)spare, 1.f);
+        if (spare == 4) return max(((int)fminf(total * 1.0005f / of, 0x1p29f) + kCut) / kCut * kCut, kMinSplit);
+        const int size = max(((int)fminf(total / of, 0x1p29f) + kCut - 1) / kCut * kCut, kMinSplit);
         int count = 0;
         for (int b0 = 0; b0 < a.batch; b0 += kWave)
             count += wave_sum(b0 + lane < a.batch ? cut_context(context(a, b0 + lane), size).ns : 0);
@@ -404,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
                 s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);  // the next loads take these registers
         after_k();
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
                 channels(v, c);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
         after_v();
     };
 
@@ -493,7 +494,11 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     Tl x;
     bool loaded = false;
     if (a.bs_shift >= 4) {
-        auto page = [&](int tok) { return tok < end ? bt[uniform(tok >> a.bs_shift)] : -1; };
+        // By scalar loads (nothing writes the table while the kernel runs): a vector
+        // load's wait would be one for all the rows in flight.
+        typedef const __attribute__((address_space(4))) int* scalar_ptr;
+        const scalar_ptr table = (scalar_ptr)(uintptr_t)bt;
+        auto page = [&](int tok) { return tok < end ? table[tok >> a.bs_shift] : -1; };
         auto whole = [&](int tile, int pa, int pb) {
             return tile + kTile <= end && (unsigned)pa < (unsigned)a.num_blocks && (unsigned)pb < (unsigned)a.num_blocks;
         };
@@ -710,14 +715,14 @@ hipError_t launch_typed(const DecodeMxArgs& x) {
 }  // namespace
 
 // Splits of a kv head over the whole batch.  Cut evenly: as many as fit the 256
-// CUs at once (four workgroups each), at least two a sequence on average, none
-// of less than kMinSplit tokens, and no more than 64 a sequence for one workgroup
-// to merge.
-int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition) {
+// CUs at once, or a quarter more than sequences (that the longest are cut), none
+// of less than kMinSplit tokens, and no more than 64 a sequence on average for one
+// workgroup to merge.
+int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t d, int64_t max_ctx, int64_t partition, bool mx) {
     if (partition > 0) return batch * ((max_ctx + partition - 1) / partition);
-    constexpr int64_t kWorkgroups = 1024, kMostSplits = 64;
-    const int64_t chunks = std::min(kMostSplits, (max_ctx + kMinSplit - 1) / kMinSplit);
-    return std::min(batch * chunks, std::max((kWorkgroups + hkv - 1) / hkv, 2 * batch));
+    const int64_t workgroups = 256 * (mx || d == 64 ? 4 : 3), most = 64;
+    const int64_t chunks = std::min(most, (max_ctx + kMinSplit - 1) / kMinSplit);
+    return std::min(batch * chunks, std::max((workgroups + hkv - 1) / hkv, batch + (batch + 3) / 4));
 }
 
 hipError_t decode_mx_launch(const DecodeMxArgs& x) {
