@@ -5,18 +5,21 @@
 // upkeep.
 //
 // evict_select_kernel, one workgroup per (sequence, kv head), bound by latency:
-// the weights as integers that order as they do; a radix select from the top
-// bits down finds the key of the last one kept (LDS histograms of 2048 bins,
-// three passes); then one pass in order of position counts those above it and
-// those equal to it before each token (ties go to the lowest positions), which
-// is its new position.
+// the weights as integers that order as they do, 16 of each of 1024 threads in
+// registers (longer contexts are read again in each pass); a radix select from the
+// top bits down finds the key of the last one kept (LDS histograms of 2048 bins,
+// three passes); then the tokens above it, and those equal to it (of which the
+// first are kept), are counted in order of position: a kept token's new position
+// is the number of kept ones before it.  Ballots count within a wave's 64 tokens,
+// one scan over the waves' counts the rest.
 //
 // evict_move_kernel, bound by memory: rows of the kept tokens are read and
 // written once.  In place, row i becomes what row kept[i] >= i was: a workgroup
 // owns a column of up to 128 bytes of one head's rows, so that no other touches
 // its bytes, reads a batch of rows, waits until all of it is read, and writes it.
 // Later batches only read rows behind what has been written, so nothing else
-// has to be ordered.
+// has to be ordered: their positions, page ids and then rows are on their way
+// before.
 #include <algorithm>
 
 #include "attn_kernels.hpp"
@@ -27,8 +30,8 @@ namespace ak {
 namespace {
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
-constexpr int kPerThread = 4;                          // consecutive tokens of a thread in a sweep
-constexpr int kSweep = kSelectThreads * kPerThread;
+constexpr int kKeys = 16;                          // of a thread, 1024 positions apart
+constexpr int kSegment = kSelectThreads * kKeys;   // tokens at a time
 constexpr int kBins = 2048;
 
 // Larger weights are larger keys; -0 equals 0, every NaN is the largest.
@@ -48,20 +51,11 @@ struct SelectParams {
     int hkv, length, max_tok, budget, recent;
 };
 
-// Sum over the workgroup of one value per wave; every thread gets it.
-__device__ __forceinline__ int wave_inclusive(int x, int lane) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int y = __shfl_up(x, d, kWave);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const SelectParams a) {
     __shared__ int hist[kBins];
     __shared__ int wave_total[kSelectWaves];
-    __shared__ int found_bin, found_above;
+    __shared__ int counts[kKeys * kSelectWaves];  // of 64 tokens each: above the key, and equal to it in the high half
+    __shared__ int found_bin, found_above, segment_total;
     const int h = blockIdx.x, b = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int n = max(min(a.ctx_lens[b], a.max_tok), 0);
@@ -69,16 +63,33 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Sele
     float* new_wt = a.new_weights + ((size_t)b * a.hkv + h) * a.length;
     int* kept = a.kept + ((size_t)b * a.hkv + h) * a.budget;
     const int m = min(n, a.budget);
+    float x[kKeys];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+            const int i = base + j * kSelectThreads + tid;
+            x[j] = i < n ? wt[i] : 0.f;
+        }
+    };
+    load(0);
     if (h == 0 && tid == 0) a.new_lens[b] = m;
     for (int i = m + tid; i < a.length; i += kSelectThreads) new_wt[i] = 0.f;
     for (int i = m + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
     if (n <= a.budget) {
-        for (int i = tid; i < n; i += kSelectThreads) {
-            kept[i] = i;
-            new_wt[i] = wt[i];
+        for (int base = 0; base < n; base += kSegment) {
+            if (base > 0) load(base);
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j) {
+                const int i = base + j * kSelectThreads + tid;
+                if (i < n) {
+                    kept[i] = i;
+                    new_wt[i] = x[j];
+                }
+            }
         }
         return;
     }
+    const bool once = n <= kSegment;  // the registers hold every token
     const int old = n - a.recent, want = a.budget - a.recent;  // 0 <= want < old
     // The key of the want-th largest of the first `old` tokens: `prefix` holds
     // its top bits, `above` of the tokens have larger ones.
@@ -93,19 +104,25 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Sele
             const int shift = kShift[pass], bins = 1 << kBits[pass];
             for (int i = tid; i < bins; i += kSelectThreads) hist[i] = 0;
             __syncthreads();
-            for (int i = tid; i < old; i += kSelectThreads) {
-                const uint32_t k = order_key(wt[i]);
-                if ((k & known) == prefix) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
+            for (int base = 0; base < old; base += kSegment) {
+                if (!once) load(base);
+#pragma unroll
+                for (int j = 0; j < kKeys; ++j) {
+                    const int i = base + j * kSelectThreads + tid;
+                    const uint32_t k = order_key(x[j]);
+                    if (i < old && (k & known) == prefix) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
+                }
             }
             __syncthreads();
             // Bins from the largest down, two of a thread: where the count passes want.
             const int hi = bins - 1 - 2 * tid;
             const int c0 = hi >= 0 ? hist[hi] : 0, c1 = hi >= 0 ? hist[hi - 1] : 0;
-            const int inc = wave_inclusive(c0 + c1, lane);
+            const int inc = wave_inclusive_sum(c0 + c1);
             if (lane == kWave - 1) wave_total[w] = inc;
             __syncthreads();
             int before = above + inc - c0 - c1;
-            for (int v = 0; v < w; ++v) before += wave_total[v];
+#pragma unroll
+            for (int v = 0; v < kSelectWaves; ++v) before += v < w ? wave_total[v] : 0;
             if (before < want && want <= before + c0) {
                 found_bin = hi;
                 found_above = before;
@@ -121,41 +138,46 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Sele
     }
     const int ties = want - above;  // tokens of that very key that are kept: the first ones (none where want is 0)
     int gt_before = 0, eq_before = 0;
-    for (int base = 0; base < n; base += kSweep) {
-        const int i0 = base + tid * kPerThread;
-        float x[kPerThread];
-        int gt[kPerThread], eq[kPerThread], packed = 0;
+    for (int base = 0; base < n; base += kSegment) {
+        if (!once) load(base);
+        uint64_t gt[kKeys], eq[kKeys];
 #pragma unroll
-        for (int j = 0; j < kPerThread; ++j) {
-            const int i = i0 + j;
-            x[j] = i < n ? wt[i] : 0.f;
+        for (int j = 0; j < kKeys; ++j) {
+            const int i = base + j * kSelectThreads + tid;
             const uint32_t k = order_key(x[j]);
-            gt[j] = i < n && (i >= old || (want > 0 && k > prefix));
-            eq[j] = i < old && want > 0 && k == prefix;
-            packed += gt[j] | eq[j] << 16;
+            gt[j] = __builtin_amdgcn_ballot_w64(i < n && (i >= old || (want > 0 && k > prefix)));
+            eq[j] = __builtin_amdgcn_ballot_w64(i < old && want > 0 && k == prefix);
+            if (lane == 0) counts[j * kSelectWaves + w] = __popcll(gt[j]) | __popcll(eq[j]) << 16;
         }
-        const int inc = wave_inclusive(packed, lane);
-        __syncthreads();  // wave_total of the sweep before has been read
-        if (lane == kWave - 1) wave_total[w] = inc;
         __syncthreads();
-        int before = inc - packed, total = 0;
-        for (int v = 0; v < kSelectWaves; ++v) {
-            if (v < w) before += wave_total[v];
-            total += wave_total[v];
-        }
-        int g = gt_before + (before & 0xffff), e = eq_before + (before >> 16);
+        if (w == 0) {  // exclusive sums over the 256 counts, four of a lane
+            int c[4], sum = 0;
 #pragma unroll
-        for (int j = 0; j < kPerThread; ++j) {
-            if (gt[j] || (eq[j] && e < ties)) {
+            for (int i = 0; i < 4; ++i) sum += c[i] = counts[4 * lane + i];
+            int before = wave_inclusive_sum(sum) - sum;
+            if (lane == kWave - 1) segment_total = before + sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                counts[4 * lane + i] = before;
+                before += c[i];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+            const int before = counts[j * kSelectWaves + w];
+            const uint64_t below = (1ull << lane) - 1;
+            const int g = gt_before + (before & 0xffff) + __popcll(gt[j] & below);
+            const int e = eq_before + (before >> 16) + __popcll(eq[j] & below);
+            if ((gt[j] >> lane & 1) || ((eq[j] >> lane & 1) && e < ties)) {
                 const int to = g + min(e, ties);
-                kept[to] = i0 + j;
+                kept[to] = base + j * kSelectThreads + tid;
                 new_wt[to] = x[j];
             }
-            g += gt[j];
-            e += eq[j];
         }
-        gt_before += total & 0xffff;
-        eq_before += total >> 16;
+        gt_before += segment_total & 0xffff;
+        eq_before += segment_total >> 16;
+        if (!once) __syncthreads();  // counts are read before the next segment's
     }
 }
 
@@ -171,37 +193,50 @@ constexpr int kMoveThreads = 256;
 constexpr int kBatch = 8;       // rows that a lane has in flight
 constexpr int kColumn = 128;    // bytes of a row that a workgroup moves
 
-// U: the bytes that a lane moves at a time.
-template <class U>
+// U: the bytes that a lane moves at a time.  POW2: pages of a power of two of tokens.
+template <class U, bool POW2>
 __device__ __forceinline__ void move_rows(const MoveParams& a, char* plane, int row_bytes, int column, int b, int h) {
     const int width = min(row_bytes - column * kColumn, kColumn) / (int)sizeof(U);  // lanes of a row
     const int tid = threadIdx.x, per_pass = kMoveThreads / width;
     const int lane_row = tid / width, offset = column * kColumn + tid % width * (int)sizeof(U);
     const bool idle = lane_row >= per_pass;
     const int m = a.new_lens[b];
+    if (m == 0) return;
     const int* kept = a.kept + ((size_t)b * a.hkv + h) * a.budget;
     const int* from = a.tables + (size_t)b * a.max_blocks;
     const int* to = a.new_tables + (size_t)b * a.new_max_blocks;
-    auto locate = [&](const int* table, int i) -> char* {  // null: no such page
-        const int pi = a.bs_shift >= 0 ? i >> a.bs_shift : i / a.bs;
-        const int page = table[pi];
-        if ((unsigned)page >= (unsigned)a.num_blocks) return nullptr;
-        return plane + (((size_t)page * a.hkv + h) * a.bs + (i - pi * a.bs)) * row_bytes + offset;
+    char* const base = plane + offset;
+    auto page_index = [&](int i) { return POW2 ? i >> a.bs_shift : i / a.bs; };
+    // Rows first, first + per_pass, ... of the batch; lanes without one take the last.
+    auto row = [&](int first, int j) { return min(first + j * per_pass + lane_row, m - 1); };
+    int src[kBatch];
+    auto positions = [&](int first) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) src[j] = kept[row(first, j)];
     };
-    for (int base = 0; base < m; base += kBatch * per_pass) {
-        U x[kBatch];
-        char* dst[kBatch];
+    positions(0);
+    const int step = kBatch * per_pass;
+    for (int first = 0; first < m; first += step) {
+        int sp[kBatch], dp[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const int i = base + j * per_pass + lane_row;
-            dst[j] = nullptr;
-            if (idle || i >= m) continue;
-            const int src = kept[i];
-            if (a.in_place && src == i) continue;
-            const char* p = locate(from, src);
-            dst[j] = p ? locate(to, i) : nullptr;
-            if (dst[j]) x[j] = *reinterpret_cast<const U*>(p);
+            sp[j] = from[page_index(src[j])];
+            dp[j] = to[page_index(row(first, j))];
         }
+        U x[kBatch];
+        char* dst[kBatch];  // null: nothing to write
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = row(first, j);
+            const bool fine = !idle && first + j * per_pass + lane_row < m && !(a.in_place && src[j] == i) &&
+                              (unsigned)sp[j] < (unsigned)a.num_blocks && (unsigned)dp[j] < (unsigned)a.num_blocks;
+            auto at = [&](int page, int token) {
+                return base + (((size_t)page * a.hkv + h) * a.bs + (token - page_index(token) * a.bs)) * row_bytes;
+            };
+            if (fine) x[j] = *reinterpret_cast<const U*>(at(sp[j], src[j]));
+            dst[j] = fine ? at(dp[j], i) : nullptr;
+        }
+        if (first + step < m) positions(first + step);
         // Every row of the batch has been read before one of them is written.
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -211,15 +246,16 @@ __device__ __forceinline__ void move_rows(const MoveParams& a, char* plane, int 
     }
 }
 
+template <bool POW2>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const MoveParams a) {
     const int h = blockIdx.y, b = blockIdx.z;
     if (a.in_place && min(a.ctx_lens[b], a.max_tok) <= a.budget) return;  // every row stays
     int plane = 0, column = blockIdx.x;
     while (column >= a.columns[plane]) column -= a.columns[plane++];
     const int rb = a.row_bytes[plane];
-    if (rb % 16 == 0) move_rows<u32x4>(a, a.rows[plane], rb, column, b, h);
-    else if (rb % 4 == 0) move_rows<uint32_t>(a, a.rows[plane], rb, column, b, h);
-    else move_rows<uint8_t>(a, a.rows[plane], rb, column, b, h);
+    if (rb % 16 == 0) move_rows<u32x4, POW2>(a, a.rows[plane], rb, column, b, h);
+    else if (rb % 4 == 0) move_rows<uint32_t, POW2>(a, a.rows[plane], rb, column, b, h);
+    else move_rows<uint8_t, POW2>(a, a.rows[plane], rb, column, b, h);
 }
 
 }  // namespace
@@ -262,8 +298,9 @@ hipError_t evict_launch(const EvictArgs& x) {
     m.new_max_blocks = (int)(x.new_block_tables ? x.new_max_blocks : x.max_blocks);
     m.num_blocks = (int)x.num_blocks;
     m.budget = (int)x.budget;
-    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)columns, (unsigned)x.hkv, (unsigned)x.batch),
-                       dim3(kMoveThreads), 0, (hipStream_t)x.stream, m);
+    auto* move = m.bs_shift >= 0 ? evict_move_kernel<true> : evict_move_kernel<false>;
+    hipLaunchKernelGGL(move, dim3((unsigned)columns, (unsigned)x.hkv, (unsigned)x.batch), dim3(kMoveThreads), 0,
+                       (hipStream_t)x.stream, m);
     return hipGetLastError();
 }
 

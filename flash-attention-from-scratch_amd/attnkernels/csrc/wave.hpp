@@ -54,6 +54,17 @@ __device__ __forceinline__ float group_sum(float x) {
     return x;
 }
 
+// Inclusive sum over the lanes of a wave (DPP row shifts, then row broadcasts).
+__device__ __forceinline__ int wave_inclusive_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);   // row_shr:2
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);   // row_shr:4
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);   // row_shr:8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return x;
+}
+
 // Value held by lane (l ^ MASK) for MASK in {8, 16, 32}: ds_swizzle / bpermute.
 template <int MASK>
 __device__ __forceinline__ float shfl_xor(float x) {
