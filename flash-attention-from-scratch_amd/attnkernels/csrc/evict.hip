@@ -64,12 +64,17 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Sele
     int* kept = a.kept + ((size_t)b * a.hkv + h) * a.budget;
     const int m = min(n, a.budget);
     float x[kKeys];
+    uint32_t key[kKeys];
+    auto some = [&](int base, int j) { return base + j * kSelectThreads < n; };  // whether any thread has a j-th token
     auto load = [&](int base) {
 #pragma unroll
         for (int j = 0; j < kKeys; ++j) {
             const int i = base + j * kSelectThreads + tid;
-            x[j] = i < n ? wt[i] : 0.f;
+            if (some(base, j)) x[j] = wt[min(i, n - 1)];
         }
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+            if (some(base, j)) key[j] = order_key(x[j]);
     };
     load(0);
     if (h == 0 && tid == 0) a.new_lens[b] = m;
@@ -108,9 +113,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Sele
                 if (!once) load(base);
 #pragma unroll
                 for (int j = 0; j < kKeys; ++j) {
+                    if (!some(base, j)) break;
                     const int i = base + j * kSelectThreads + tid;
-                    const uint32_t k = order_key(x[j]);
-                    if (i < old && (k & known) == prefix) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
+                    if (i < old && (key[j] & known) == prefix) atomicAdd(&hist[key[j] >> shift & (bins - 1)], 1);
                 }
             }
             __syncthreads();
@@ -144,7 +149,12 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Sele
 #pragma unroll
         for (int j = 0; j < kKeys; ++j) {
             const int i = base + j * kSelectThreads + tid;
-            const uint32_t k = order_key(x[j]);
+            const uint32_t k = key[j];
+            gt[j] = eq[j] = 0;
+            if (!some(base, j)) {
+                if (lane == 0) counts[j * kSelectWaves + w] = 0;
+                continue;
+            }
             gt[j] = __builtin_amdgcn_ballot_w64(i < n && (i >= old || (want > 0 && k > prefix)));
             eq[j] = __builtin_amdgcn_ballot_w64(i < old && want > 0 && k == prefix);
             if (lane == 0) counts[j * kSelectWaves + w] = __popcll(gt[j]) | __popcll(eq[j]) << 16;
@@ -165,6 +175,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Sele
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < kKeys; ++j) {
+            if (!some(base, j)) break;
             const int before = counts[j * kSelectWaves + w];
             const uint64_t below = (1ull << lane) - 1;
             const int g = gt_before + (before & 0xffff) + __popcll(gt[j] & below);
