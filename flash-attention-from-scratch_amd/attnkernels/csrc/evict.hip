@@ -17,9 +17,8 @@
 // written once.  In place, row i becomes what row kept[i] >= i was: a workgroup
 // owns a column of up to 128 bytes of one head's rows, so that no other touches
 // its bytes, reads a batch of rows, waits until all of it is read, and writes it.
-// Later batches only read rows behind what has been written, so nothing else
-// has to be ordered: their positions, page ids and then rows are on their way
-// before.
+// Later batches only read rows behind what is written before them, so nothing else
+// has to be ordered, and the next batch is on its way meanwhile.
 #include <algorithm>
 
 #include "attn_kernels.hpp"
@@ -220,22 +219,23 @@ __device__ __forceinline__ void move_rows(const MoveParams& a, char* plane, int 
     auto page_index = [&](int i) { return POW2 ? i >> a.bs_shift : i / a.bs; };
     // Rows first, first + per_pass, ... of the batch; lanes without one take the last.
     auto row = [&](int first, int j) { return min(first + j * per_pass + lane_row, m - 1); };
-    int src[kBatch];
+    int src[kBatch];  // positions of the batch to be read next
     auto positions = [&](int first) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) src[j] = kept[row(first, j)];
     };
-    positions(0);
     const int step = kBatch * per_pass;
-    for (int first = 0; first < m; first += step) {
+    struct Rows {
+        U x[kBatch];
+        char* dst[kBatch];  // null: nothing to write
+    };
+    auto read = [&](Rows& r, int first) {
         int sp[kBatch], dp[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             sp[j] = from[page_index(src[j])];
             dp[j] = to[page_index(row(first, j))];
         }
-        U x[kBatch];
-        char* dst[kBatch];  // null: nothing to write
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const int i = row(first, j);
@@ -244,16 +244,38 @@ __device__ __forceinline__ void move_rows(const MoveParams& a, char* plane, int 
             auto at = [&](int page, int token) {
                 return base + (((size_t)page * a.hkv + h) * a.bs + (token - page_index(token) * a.bs)) * row_bytes;
             };
-            if (fine) x[j] = *reinterpret_cast<const U*>(at(sp[j], src[j]));
-            dst[j] = fine ? at(dp[j], i) : nullptr;
+            r.x[j] = U{};
+            if (fine) r.x[j] = *reinterpret_cast<const U*>(at(sp[j], src[j]));
+            r.dst[j] = fine ? at(dp[j], i) : nullptr;
         }
         if (first + step < m) positions(first + step);
-        // Every row of the batch has been read before one of them is written.
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+    };
+    auto write = [&](const Rows& r) {
+        // Every row of the batch has been read, by all waves, before one of them is
+        // written: the use of r.x waits for this wave's (but not for the next batch's).
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if constexpr (sizeof(U) < 4) asm volatile("" ::"v"((uint32_t)r.x[j]) : "memory");
+            else asm volatile("" ::"v"(r.x[j]) : "memory");
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
-            if (dst[j]) *reinterpret_cast<U*>(dst[j]) = x[j];
+            if (r.dst[j]) *reinterpret_cast<U*>(r.dst[j]) = r.x[j];
+    };
+    // A batch is read while the one before is written: what it reads lies behind
+    // all that is written by then.
+    Rows p, q;
+    positions(0);
+    read(p, 0);
+    for (int first = 0;;) {
+        if ((first += step) < m) read(q, first);
+        write(p);
+        if (first >= m) break;
+        if ((first += step) < m) read(p, first);
+        write(q);
+        if (first >= m) break;
     }
 }
 
