@@ -7,7 +7,8 @@
 //
 // A weight needs its whole row's maximum and sum, so the scores are formed
 // twice, each time by the same tile product on 32x32x16 MFMAs: 64 columns a
-// wave stay in registers, tiles of 64 rows pass through LDS.
+// wave (32 where there is little work) stay in registers, tiles of 64 rows pass
+// through LDS.
 //   * prompt_stats_kernel holds queries and streams the keys up to them: per
 //     query the running maximum and the sum of exponentials.  A workgroup's four
 //     waves hold consecutive (64 queries, head) chunks of one kv head, heads
@@ -30,11 +31,18 @@ namespace ak {
 namespace {
 
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
-constexpr int kCols = 64;             // columns that a wave holds
-constexpr int kHeld = kWaves * kCols; // of a workgroup
+template <int C>
+constexpr int kCols = 32 * C;             // columns that a wave holds
+template <int C>
+constexpr int kHeld = kWaves * kCols<C>;  // of a workgroup
 constexpr int kTile = 64;             // rows of a streamed tile
 constexpr int kRing = 3;              // tiles in LDS: one in use, two on their way
 constexpr int kRows = 512;            // queries whose maxima and sums a workgroup of the second pass has in LDS
+// Wave tiles from which on a wave holds 64 columns.  Measured with 64 / 32 columns,
+// us, Hq=32, Hkv=8, D=128, all queries: 512 tokens (2048 tiles) 29.1 / 23.9, 1111
+// (10368) 44.8 / 42.0, 1500 (18432) 54.3 / 49.3, 2048 (32768) 83.5 / 85.0, 8192
+// (524288) 687 / 742; 12 x 4096, the last 64 (24576) 89.5 / 95.0.
+constexpr double kManyTiles = 20000;
 constexpr float kLowest = -3.402823466e38f;
 
 struct Params {
@@ -42,10 +50,11 @@ struct Params {
     const int* cu;
     float* weights;
     float *m, *l;          // [key splits, hq, total]
-    float* partial;        // [items, hkv, total]
+    float* partial;        // [items, hkv, total]; nullptr: one item, written to weights
     int64_t q_stride, k_stride, w_stride_b, w_stride_h;
     int total, hkv, group, max_seqlen, last, length;
     int key_range, key_splits, heads, items_h, row_range, ranges;
+    int held;             // keys of a workgroup of the second pass
     int pairs, key_tiles;  // (sequence, kv head) pairs, the fastest part of a workgroup's number: one's keys meet in one L2
     float sl2;
 };
@@ -125,39 +134,39 @@ __device__ __forceinline__ float masked_score(float sl2) { return sl2 < 0.f ? IN
 // The order of a stage's instructions (0x008 MFMA, 0x002 vector, 0x400
 // exponentials, 0x100 LDS reads): the products of one block with an equal share
 // of the other's exponentials and VALU vector instructions behind each.
-template <int D, int VALU>
+template <int D, int C, int VALU>
 __device__ __forceinline__ void interleave() {
-    constexpr int N = D / 8;  // products
+    constexpr int N = C * D / 16;  // products
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x002, (VALU + N - 1) / N, 0);
-        __builtin_amdgcn_sched_group_barrier(0x400, 32 / N, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 16 * C / N, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
 }
 
 // Scores (unscaled) of the tile's rows 32 blk .. 32 blk + 31 against the held columns.
-template <int D, class T>
-__device__ __forceinline__ void product(const u32x4* tile, int blk, const u32x4 (&held)[2][D / 16], int lane,
-                                        f32x16 (&s)[2]) {
+template <int D, class T, int C>
+__device__ __forceinline__ void product(const u32x4* tile, int blk, const u32x4 (&held)[C][D / 16], int lane,
+                                        f32x16 (&s)[C]) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[c][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
         const u32x4 row = tile[place<D>(32 * blk + (lane & 31), 2 * k + (lane >> 5))];
-        s[0] = Half<T>::mfma32(row, held[0][k], s[0]);
-        s[1] = Half<T>::mfma32(row, held[1][k], s[1]);
+#pragma unroll
+        for (int c = 0; c < C; ++c) s[c] = Half<T>::mfma32(row, held[c][k], s[c]);
     }
 }
 
-template <int D>
-__device__ __forceinline__ void hold(const Rows& rows, int i0, int end, int lane, u32x4 (&held)[2][D / 16]) {
+template <int D, int C>
+__device__ __forceinline__ void hold(const Rows& rows, int i0, int end, int lane, u32x4 (&held)[C][D / 16]) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
         const int i = min(i0 + 32 * c + (lane & 31), end - 1);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
@@ -168,38 +177,43 @@ __device__ __forceinline__ void hold(const Rows& rows, int i0, int end, int lane
 // The row of register r of a 32 x 32 product in this lane.
 __device__ __forceinline__ int row_of(int r, int lane) { return 8 * (r / 4) + 4 * (lane >> 5) + r % 4; }
 
-template <int D, class T>
-__global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params a) {
+template <int D, class T, int C>
+__global__ void __launch_bounds__(kThreads, C == 2 ? 2 : 3) prompt_stats_kernel(const Params a) {
     __shared__ u32x4 tiles[kRing][kTile * kUnits<D>];
     const int pair = blockIdx.x % a.pairs, kvh = pair % a.hkv, b = pair / a.hkv;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int G = a.group;
     const Sequence sq = sequence(a, b);
     const int R = sq.n - sq.first;
-    const int chunks = (R + kCols - 1) / kCols * G;
+    const int chunks = (R + kCols<C> - 1) / kCols<C> * G;
     // The longest streams first: the last queries have the lowest workgroup numbers.
     const int groups = (chunks + kWaves - 1) / kWaves, index = blockIdx.x / a.pairs;
     const int part = index % a.key_splits, group = groups - 1 - index / a.key_splits;
     if (group < 0) return;
     const int chunk = min(group * kWaves + w, chunks - 1);
-    const int h = kvh * G + chunk % G, q0 = sq.first + chunk / G * kCols;  // position of the wave's first query
+    const int h = kvh * G + chunk % G, q0 = sq.first + chunk / G * kCols<C>;  // position of the wave's first query
     const bool spare = group * kWaves + w >= chunks;
     const int last_chunk = min(group * kWaves + kWaves, chunks) - 1;
     const int begin = part * a.key_range;
-    const int end = min(min(sq.first + (last_chunk / G + 1) * kCols, sq.n), begin + a.key_range);
+    const int end = min(min(sq.first + (last_chunk / G + 1) * kCols<C>, sq.n), begin + a.key_range);
     const int count = begin < end ? (end - begin + kTile - 1) / kTile : 0;
     const Rows keys{a.k + (int64_t)sq.start * a.k_stride + kvh * D, a.k_stride};
     const Rows queries{a.q + (int64_t)sq.start * a.q_stride + h * D, a.q_stride};
     for (int t = 0; t < kRing - 1 && t < count; ++t) load_tile<D>(keys, begin + t * kTile, end, tiles[t], w, lane);
-    u32x4 held[2][D / 16];
-    hold<D>(queries, q0, sq.n, lane, held);
+    u32x4 held[C][D / 16];
+    hold<D, C>(queries, q0, sq.n, lane, held);
 
     const float lowest = masked_score(a.sl2);
-    float m[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f};
-    // Adds the exponentials of a block's scores to sum.
-    auto weigh = [&](const f32x16 (&x)[2], float (&sum)[2]) {
+    float m[C], l[C];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
+        m[c] = kLowest;
+        l[c] = 0.f;
+    }
+    // Adds the exponentials of a block's scores to sum.
+    auto weigh = [&](const f32x16 (&x)[C], float (&sum)[C]) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
             float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int r = 0; r < 16; ++r) t[r % 4] += exp2_fast(x[c][r] * a.sl2 - m[c]);
@@ -209,24 +223,26 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params 
     // One stage: the scores of rows kb .. (tile block blk) into x, while those of
     // the block before, y, become exponentials; live: the block before has any.
     bool live = false;
-    auto stage = [&](const u32x4* tile, int blk, int kb, f32x16 (&x)[2], const f32x16 (&y)[2]) {
-        const bool now = !spare && kb < end && kb < q0 + kCols;  // a key that some query sees
-        float sum[2];
+    auto stage = [&](const u32x4* tile, int blk, int kb, f32x16 (&x)[C], const f32x16 (&y)[C]) {
+        const bool now = !spare && kb < end && kb < q0 + kCols<C>;  // a key that some query sees
+        float sum[C];
         if (now && live) {
-            product<D, T>(tile, blk, held, lane, x);
+            product<D, T, C>(tile, blk, held, lane, x);
             weigh(y, sum);
-            interleave<D, 32 * 2 + 8>();
+            interleave<D, C, C * 36>();
         } else if (now) {
-            product<D, T>(tile, blk, held, lane, x);
+            product<D, T, C>(tile, blk, held, lane, x);
         } else if (live) {
             weigh(y, sum);
         }
         if (live) {
             // The maximum subtracted stays unless the sums pass 2^100 (as
             // against the lowest number at first); then the block is done again.
-            if (__builtin_amdgcn_ballot_w64(!(sum[0] <= 0x1p100f) || !(sum[1] <= 0x1p100f))) {
+            float top = sum[0];
+            if constexpr (C == 2) top += sum[1];
+            if (__builtin_amdgcn_ballot_w64(!(top <= 0x1p100f))) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < C; ++c) {
                     float mx = m[c];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[c][r] * a.sl2);
@@ -235,12 +251,12 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params 
                 }
                 weigh(y, sum);
             }
-            l[0] = sum[0];
-            l[1] = sum[1];
+#pragma unroll
+            for (int c = 0; c < C; ++c) l[c] = sum[c];
         }
         if (now && (kb + 31 > q0 || kb + 32 > end)) {  // keys after a query, or past the range
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < C; ++c) {
                 int limit = min(q0 + 32 * c + (lane & 31), end - 1) - kb;
                 asm volatile("" : "+v"(limit));  // nothing of this is done ahead of the branch
 #pragma unroll
@@ -249,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params 
         }
         live = now;
     };
-    f32x16 x[2], y[2];
+    f32x16 x[C], y[C];
     for (int t = 0, cur = 0; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
         const int k0 = begin + t * kTile;
         tile_ready<D>(count - 1 - t);
@@ -262,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params 
     if (spare) return;
     // A column's rows are in two lanes.
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
         const float m2 = __shfl_xor(m[c], 32, kWave), l2 = __shfl_xor(l[c], 32, kWave);
         const float mx = fmaxf(m[c], m2);
         const float sum = l[c] * exp2_fast(m[c] - mx) + l2 * exp2_fast(m2 - mx);
@@ -275,14 +291,14 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_stats_kernel(const Params 
     }
 }
 
-// Whether the queries of range j reach key tile kt (tiles of kHeld keys).
-__device__ __forceinline__ bool reaches(const Params& a, const Sequence& sq, int j, int kt) {
+// Whether the queries of range j reach a tile of keys that begins with `key`.
+__device__ __forceinline__ bool reaches(const Params& a, const Sequence& sq, int j, int key) {
     const int lo = sq.first + j * a.row_range, hi = min(sq.n, lo + a.row_range);
-    return lo < hi && hi > kt * kHeld;
+    return lo < hi && hi > key;
 }
 
-template <int D, class T>
-__global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a) {
+template <int D, class T, int C>
+__global__ void __launch_bounds__(kThreads, C == 2 ? 2 : 3) prompt_sums_kernel(const Params a) {
     __shared__ u32x4 tiles[kRing][kTile * kUnits<D>];
     __shared__ f32x4 row_m[kRows / 4], row_w[kRows / 4];
     // The last ranges, which all keys stream, first.
@@ -293,11 +309,16 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
     const int kt = index % a.key_tiles, j = a.ranges - 1 - index / a.key_tiles, item = part * a.ranges + j;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const Sequence sq = sequence(a, b);
-    if (kt * kHeld >= sq.n || !reaches(a, sq, j, kt)) return;
+    const int k0 = kt * kHeld<C> + w * kCols<C>;
+    // One item in all: its sums are the weights.
+    float* const weights = a.partial ? nullptr : a.weights + b * a.w_stride_b + kvh * a.w_stride_h;
+    if (kt * kHeld<C> >= sq.n || !reaches(a, sq, j, kt * kHeld<C>)) {
+        if (weights && lane < kCols<C> && k0 + lane < a.length) weights[k0 + lane] = 0.f;
+        return;
+    }
     const int heads = min(a.heads, a.group - head0), h0 = kvh * a.group + head0;
-    const int k0 = kt * kHeld + w * kCols;
     const int lo = sq.first + j * a.row_range, end = min(sq.n, lo + a.row_range);
-    const int begin = lo + max(kt * kHeld - lo, 0) / kTile * kTile;
+    const int begin = lo + max(kt * kHeld<C> - lo, 0) / kTile * kTile;
     const int per_head = (end - begin + kTile - 1) / kTile, count = per_head * heads;
     const Rows keys{a.k + (int64_t)sq.start * a.k_stride + kvh * D, a.k_stride};
     Rows queries{a.q + (int64_t)sq.start * a.q_stride + (int64_t)h0 * D, a.q_stride};
@@ -311,8 +332,8 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
         }
     };
     for (int t = 0; t < kRing - 1 && t < count; ++t) load_next(t);
-    u32x4 held[2][D / 16];
-    hold<D>(keys, k0, sq.n, lane, held);
+    u32x4 held[C][D / 16];
+    hold<D, C>(keys, k0, sq.n, lane, held);
     // Every row's maximum and 1 / sum over the key splits; rows past the end weigh nothing.
     for (int i = tid; i < count * kTile; i += kThreads) {
         const int head = i / (per_head * kTile), pos = begin + i % (per_head * kTile);
@@ -344,14 +365,14 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
         reinterpret_cast<float*>(row_w)[i] = wgt;
     }
     const float lowest = masked_score(a.sl2);
-    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    float sum[C][2] = {};
     // Adds a block's weights; its rows' numbers among row_m and row_w start at 32 at.
-    auto weigh = [&](const f32x16 (&x)[2], int at) {
+    auto weigh = [&](const f32x16 (&x)[C], int at) {
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const f32x4 m = row_m[8 * at + r / 2 + (lane >> 5)], wgt = row_w[8 * at + r / 2 + (lane >> 5)];
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     sum[c][i % 2] = fmaf(exp2_fast(x[c][r + i] * a.sl2 - m[i]), wgt[i], sum[c][i % 2]);
@@ -359,20 +380,20 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
     };
     // One stage, as in the first pass: rows ib .. , the at-th block.
     bool live = false;
-    auto stage = [&](const u32x4* tile, int blk, int ib, int at, f32x16 (&x)[2], const f32x16 (&y)[2]) {
+    auto stage = [&](const u32x4* tile, int blk, int ib, int at, f32x16 (&x)[C], const f32x16 (&y)[C]) {
         const bool now = ib < end && ib + 32 > k0;  // a query that sees some key
         if (now && live) {
-            product<D, T>(tile, blk, held, lane, x);
+            product<D, T, C>(tile, blk, held, lane, x);
             weigh(y, at - 1);
-            interleave<D, 32 * 2>();
+            interleave<D, C, C * 32>();
         } else if (now) {
-            product<D, T>(tile, blk, held, lane, x);
+            product<D, T, C>(tile, blk, held, lane, x);
         } else if (live) {
             weigh(y, at - 1);
         }
-        if (now && ib < k0 + kCols - 1) {  // queries before a key
+        if (now && ib < k0 + kCols<C> - 1) {  // queries before a key
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < C; ++c) {
                 int limit = k0 + 32 * c + (lane & 31) - ib;
                 asm volatile("" : "+v"(limit));  // nothing of this is done ahead of the branch
 #pragma unroll
@@ -381,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
         }
         live = now;
     };
-    f32x16 x[2], y[2];
+    f32x16 x[C], y[C];
     for (int t = 0, cur = 0, i0 = begin; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
         tile_ready<D>(count - 1 - t);
         if (t + kRing - 1 < count) load_next(cur == 0 ? kRing - 1 : cur - 1);
@@ -392,10 +413,12 @@ __global__ void __launch_bounds__(kThreads, 2) prompt_sums_kernel(const Params a
     }
     stage(tiles[0], 0, end, 2 * count, x, y);  // the last block's weights
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
         const float one = sum[c][0] + sum[c][1], both = one + __shfl_xor(one, 32, kWave);
         const int i = k0 + 32 * c + (lane & 31);
-        if (lane < 32 && i < sq.n) a.partial[((size_t)item * a.hkv + kvh) * a.total + sq.start + i] = both;
+        if (lane >= 32) continue;
+        if (weights && i < a.length) weights[i] = i < sq.n ? both : 0.f;
+        if (!weights && i < sq.n) a.partial[((size_t)item * a.hkv + kvh) * a.total + sq.start + i] = both;
     }
 }
 
@@ -406,7 +429,7 @@ __global__ void __launch_bounds__(kThreads) prompt_join_kernel(const Params a) {
     float sum = 0.f;
     if (i < sq.n) {
         // The ranges whose queries reach the token's tile are the last ones.
-        const int used = (sq.n - sq.first + a.row_range - 1) / a.row_range, tile = i / kHeld * kHeld;
+        const int used = (sq.n - sq.first + a.row_range - 1) / a.row_range, tile = i / a.held * a.held;
         const int j0 = min(max((tile - sq.first) / a.row_range, 0), used);
         const float* p = a.partial + (size_t)kvh * a.total + sq.start + i;
         const size_t step = (size_t)a.hkv * a.total;
@@ -417,47 +440,51 @@ __global__ void __launch_bounds__(kThreads) prompt_join_kernel(const Params a) {
     a.weights[b * a.w_stride_b + kvh * a.w_stride_h + i] = sum;
 }
 
-// How the work is cut.  First pass: keys are split where few queries count, for
-// two workgroups a CU.  Second pass: an item is a range of at most kRows queries
-// of one head, or several heads' queries where a head has few of them and enough
-// workgroups are left.
+// How the work is cut.  A wave holds 64 columns (C = 2), or 32 where workgroups are
+// few: more of them, and of fewer registers, then hide each other's latencies.
+// First pass: keys are split where few queries count.  Second pass: an item is a
+// range of at most kRows queries of one head, or several heads' queries where a
+// head has few of them and enough workgroups are left.
 struct Plan {
+    int64_t columns;  // C
     int64_t key_range, key_splits, heads, items_h, row_range, ranges;
+    int64_t key_tiles, stats_workgroups, sums_workgroups;
 };
 
-Plan make_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t max_seqlen, int64_t last) {
+Plan make_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t max_seqlen, int64_t last, int64_t length) {
     Plan p;
-    const int64_t rows = std::min(last, max_seqlen), group = hq / hkv, per_group = batch * hkv;
-    const int64_t groups = ((rows + kCols - 1) / kCols * group + kWaves - 1) / kWaves;
+    const int64_t rows = std::min(last, max_seqlen), group = hq / hkv, pairs = batch * hkv;
+    auto groups_of = [&](int64_t columns) {
+        return ((rows + 32 * columns - 1) / (32 * columns) * group + kWaves - 1) / kWaves;
+    };
+    // Wave tiles of 64 columns and 64 rows, counted as if no mask cut them.
+    const double tiles = (double)batch * hq * ((rows + 63) / 64) * ((max_seqlen + 63) / 64);
+    p.columns = tiles >= kManyTiles ? 2 : 1;
+    const int64_t slots = p.columns == 2 ? 512 : 768, groups = groups_of(p.columns);
     const int64_t most = (max_seqlen + 127) / 128;  // ranges of at least 128 keys
-    const int64_t want = std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(1, groups * per_group)));
+    const int64_t want = std::max<int64_t>(1, std::min(most, slots / std::max<int64_t>(1, groups * pairs)));
     p.key_range = ((max_seqlen + want - 1) / want + kTile - 1) / kTile * kTile;
     p.key_splits = (max_seqlen + p.key_range - 1) / p.key_range;
     p.row_range = kRows;
     p.ranges = (rows + kRows - 1) / kRows;
     p.heads = 1;
+    const int64_t held = kWaves * 32 * p.columns, key_tiles = (max_seqlen + held - 1) / held;
     if (p.ranges == 1) {
-        const int64_t padded = (rows + kTile - 1) / kTile * kTile, tiles = (max_seqlen + kHeld - 1) / kHeld;
+        const int64_t padded = (rows + kTile - 1) / kTile * kTile;
         while (p.heads * 2 <= group && p.heads * 2 * padded <= kRows &&
-               tiles * per_group * ((group + p.heads * 2 - 1) / (p.heads * 2)) >= 512)
+               key_tiles * pairs * ((group + p.heads * 2 - 1) / (p.heads * 2)) >= slots)
             p.heads *= 2;
     }
     p.items_h = (group + p.heads - 1) / p.heads;
+    // One item writes the weights itself, the zeros behind the longest prompt too.
+    p.key_tiles = p.items_h * p.ranges == 1 ? (length + held - 1) / held : key_tiles;
+    p.stats_workgroups = groups * p.key_splits * pairs;
+    p.sums_workgroups = p.key_tiles * p.items_h * p.ranges * pairs;
     return p;
 }
 
-int64_t stats_workgroups(const Plan& p, const PromptWeightsArgs& x) {
-    const int64_t groups = ((x.last + kCols - 1) / kCols * (x.hq / x.hkv) + kWaves - 1) / kWaves;
-    return groups * p.key_splits * x.batch * x.hkv;
-}
-
-int64_t sums_workgroups(const Plan& p, const PromptWeightsArgs& x) {
-    return (x.max_seqlen + kHeld - 1) / kHeld * p.items_h * p.ranges * x.batch * x.hkv;
-}
-
-template <int D, class T>
-hipError_t launch(const PromptWeightsArgs& x) {
-    const Plan plan = make_plan(x.batch, x.hq, x.hkv, x.max_seqlen, x.last);
+template <int D, class T, int C>
+hipError_t launch(const PromptWeightsArgs& x, const Plan& plan) {
     Params p{};
     p.q = static_cast<const uint16_t*>(x.q);
     p.k = static_cast<const uint16_t*>(x.k);
@@ -466,7 +493,8 @@ hipError_t launch(const PromptWeightsArgs& x) {
     const size_t stats = (size_t)plan.key_splits * x.hq * x.total;
     p.m = static_cast<float*>(x.workspace);
     p.l = p.m + stats;
-    p.partial = p.l + stats;
+    const bool direct = plan.items_h * plan.ranges == 1;
+    p.partial = direct ? nullptr : p.l + stats;
     p.q_stride = x.q_stride;
     p.k_stride = x.k_stride;
     p.w_stride_b = x.w_stride_b;
@@ -474,8 +502,8 @@ hipError_t launch(const PromptWeightsArgs& x) {
     p.total = (int)x.total;
     p.hkv = (int)x.hkv;
     p.group = (int)(x.hq / x.hkv);
-    p.max_seqlen = (int)std::min(x.max_seqlen, x.total);
-    p.last = (int)std::min(x.last, x.max_seqlen);
+    p.max_seqlen = (int)x.max_seqlen;
+    p.last = (int)x.last;
     p.length = (int)x.length;
     p.key_range = (int)plan.key_range;
     p.key_splits = (int)plan.key_splits;
@@ -484,24 +512,31 @@ hipError_t launch(const PromptWeightsArgs& x) {
     p.row_range = (int)plan.row_range;
     p.ranges = (int)plan.ranges;
     p.sl2 = x.sl2;
+    p.held = kHeld<C>;
     p.pairs = (int)(x.batch * x.hkv);
-    p.key_tiles = (int)((x.max_seqlen + kHeld - 1) / kHeld);
+    p.key_tiles = (int)plan.key_tiles;
     const auto stream = (hipStream_t)x.stream;
-    const unsigned hkv = (unsigned)x.hkv, batch = (unsigned)x.batch;
-    hipLaunchKernelGGL((prompt_stats_kernel<D, T>), dim3((unsigned)stats_workgroups(plan, x)), dim3(kThreads), 0, stream,
+    hipLaunchKernelGGL((prompt_stats_kernel<D, T, C>), dim3((unsigned)plan.stats_workgroups), dim3(kThreads), 0, stream,
                        p);
-    hipLaunchKernelGGL((prompt_sums_kernel<D, T>), dim3((unsigned)sums_workgroups(plan, x)), dim3(kThreads), 0, stream,
-                       p);
-    hipLaunchKernelGGL(prompt_join_kernel, dim3((unsigned)((x.length + kThreads - 1) / kThreads), hkv, batch),
+    hipLaunchKernelGGL((prompt_sums_kernel<D, T, C>), dim3((unsigned)plan.sums_workgroups), dim3(kThreads), 0, stream, p);
+    if (direct) return hipGetLastError();
+    hipLaunchKernelGGL(prompt_join_kernel,
+                       dim3((unsigned)((x.length + kThreads - 1) / kThreads), (unsigned)x.hkv, (unsigned)x.batch),
                        dim3(kThreads), 0, stream, p);
     return hipGetLastError();
+}
+
+template <int D, class T>
+hipError_t launch_columns(const PromptWeightsArgs& x) {
+    const Plan plan = make_plan(x.batch, x.hq, x.hkv, x.max_seqlen, x.last, x.length);
+    return plan.columns == 2 ? launch<D, T, 2>(x, plan) : launch<D, T, 1>(x, plan);
 }
 
 }  // namespace
 
 size_t prompt_weights_workspace(int64_t batch, int64_t total, int64_t hq, int64_t hkv, int64_t max_seqlen,
                                 int64_t last) {
-    const Plan p = make_plan(batch, hq, hkv, max_seqlen, last);
+    const Plan p = make_plan(batch, hq, hkv, max_seqlen, last, max_seqlen);
     return sizeof(float) * (size_t)total * (size_t)(2 * p.key_splits * hq + hkv * p.items_h * p.ranges);
 }
 
@@ -518,14 +553,14 @@ hipError_t prompt_weights_launch(const PromptWeightsArgs& x) {
                            dim3(kThreads), 0, (hipStream_t)x.stream, p);
         return hipGetLastError();
     }
-    if (x.d == 128) return x.bf16 ? launch<128, bf16>(x) : launch<128, f16>(x);
-    return x.bf16 ? launch<64, bf16>(x) : launch<64, f16>(x);
+    if (x.d == 128) return x.bf16 ? launch_columns<128, bf16>(x) : launch_columns<128, f16>(x);
+    return x.bf16 ? launch_columns<64, bf16>(x) : launch_columns<64, f16>(x);
 }
 
 bool prompt_weights_fits(const PromptWeightsArgs& x) {
     if (x.total == 0 || x.max_seqlen == 0) return true;
-    const Plan p = make_plan(x.batch, x.hq, x.hkv, x.max_seqlen, x.last);
-    return std::max(stats_workgroups(p, x), sums_workgroups(p, x)) <= INT32_MAX;
+    const Plan p = make_plan(x.batch, x.hq, x.hkv, x.max_seqlen, x.last, x.length);
+    return std::max(p.stats_workgroups, p.sums_workgroups) <= INT32_MAX;
 }
 
 }  // namespace ak
