@@ -117,7 +117,7 @@ struct DecodeMxArgs {
 hipError_t cache_write_mxfp4_launch(const CacheMxArgs& a);
 hipError_t cache_read_mxfp4_launch(const CacheMxArgs& a);
 hipError_t decode_mx_launch(const DecodeMxArgs& a);
-int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition);
+int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition, int64_t row_bytes);
 
 // Eviction by accumulated weight (evict.hip).
 struct EvictArgs {

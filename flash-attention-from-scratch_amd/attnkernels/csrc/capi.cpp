@@ -233,7 +233,8 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
     if (max_context_len > INT_MAX / 2 || partition > INT_MAX / 2 || num_blocks > INT_MAX ||
         max_blocks_per_seq > INT_MAX / 2 / block_size || batch > 65535 || num_kv_heads > 65535)
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": size out of range");
-    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition);
+    const int64_t row_bytes = k_scales ? head_dim * 17 / 16 : 4 * head_dim;
+    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition, row_bytes);
     if (slots > INT_MAX / num_kv_heads) return fail(AK_ERR_INVALID_ARGUMENT, who + ": too many splits");
     if (weights) {
         if (w_length < max_context_len)
@@ -563,7 +564,8 @@ size_t ak_paged_decode_mx_workspace_size(int64_t batch, int64_t num_heads, int64
     if (batch < 1 || num_heads < 1 || num_kv_heads < 1 || head_dim <= 0 || max_context_len < 1 || partition < 0 ||
         max_context_len > INT_MAX / 2)
         return 0;
-    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition);
+    // As for 16-bit caches, which are cut into as many splits as 4-bit ones or more.
+    const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition, 4 * head_dim);
     if (slots <= batch && !with_weights) return 0;
     const size_t parts = partials_bytes(1, num_heads, slots, head_dim) + (size_t)batch * 2 * sizeof(int32_t) + 8;
     return with_weights ? round16(parts) + (size_t)batch * (size_t)num_heads * (size_t)scores_row(max_context_len) *

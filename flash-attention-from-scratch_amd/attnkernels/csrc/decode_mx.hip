@@ -30,6 +30,7 @@
 #include <algorithm>
 
 #include "attn_kernels.hpp"
+#include "index_math.hpp"
 #include "mxfp4.hpp"
 
 #include <type_traits>
@@ -81,11 +82,16 @@ __device__ __forceinline__ f32x4 coherent_load4(const float* p) {  // 8-byte ali
 struct Cut {
     int ns, piece;
 };
-__device__ __forceinline__ Cut cut_context(int len, int size) {
-    const int n = max((len + size - 1) / size, 1);
+__device__ __forceinline__ int parts(int len, int size, int max_tok) {
+    return max_tok < 1 << 24 ? split_count(len, size, __builtin_amdgcn_rcpf((float)size)) : (len + size - 1) / size;
+}
+__device__ __forceinline__ Cut cut_context(int len, int size, int max_tok) {
+    const int n = max(parts(len, size, max_tok), 1);
     Cut c;
-    c.piece = max(((len + n - 1) / n + kCut - 1) / kCut * kCut, kCut);
-    c.ns = max((len + c.piece - 1) / c.piece, 1);
+    // At least ceil(len / n), or n would not do: the approximate quotient is off by 1.5 at most, its whole part by 2.5.
+    const int each = max_tok < 1 << 24 ? (int)((float)len * __builtin_amdgcn_rcpf((float)n)) + 3 : (len + n - 1) / n;
+    c.piece = max((min(each, size) + kCut - 1) / kCut * kCut, kCut);
+    c.ns = max(parts(len, c.piece, max_tok), 1);
     return c;
 }
 
@@ -100,44 +106,44 @@ __device__ __forceinline__ int wave_sum(int x) {
            __builtin_amdgcn_readlane(x, 63);
 }
 
-// Tokens per split.  Cut evenly: the smallest of five sizes whose splits fit the
-// slots; the last one always does: sum ceil(len / size) <= sum len / size + batch.
-__device__ __forceinline__ int split_size(const Params& a, int lane) {
-    if (a.partition > 0) return a.partition;
-    if (a.slots <= a.batch) return INT32_MAX / 4 / kCut * kCut;  // a split each
-    float total = 0.f;  // in units of 64 tokens, rounded up, so that 64 of them fit an integer
-    for (int b0 = 0; b0 < a.batch; b0 += kWave)
-        total += (float)wave_sum(b0 + lane < a.batch ? (context(a, b0 + lane) + 63) / 64 : 0) * 64.f;
-    for (int spare = 0;; ++spare) {
-        const float of = fmaxf((float)a.slots - (float)a.batch * 0.25f * (float)spare, 1.f);
-        if (spare == 4) return max(((int)fminf(total * 1.0005f / of, 0x1p29f) + kCut) / kCut * kCut, kMinSplit);
-        const int size = max(((int)fminf(total / of, 0x1p29f) + kCut - 1) / kCut * kCut, kMinSplit);
-        int count = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += kWave)
-            count += wave_sum(b0 + lane < a.batch ? cut_context(context(a, b0 + lane), size).ns : 0);
-        if (count <= a.slots) return size;
-    }
-}
-
-// The split that slot `slot` holds: every wave counts the splits of the sequences
-// in order.  b < 0: none.
+// The split that slot `slot` holds.  b < 0: none.
 struct Segment {
     int b, split, ns, piece, first, ctx;  // first: the sequence's first slot
 };
 __device__ __forceinline__ Segment segment(const Params& a, int slot, int lane) {
+    // Contexts of 64 sequences a lane each; those of the first 64 are kept.
+    const int ctx0 = lane < a.batch ? context(a, lane) : 0;
+    auto ctx_of = [&](int b0) { return b0 == 0 ? ctx0 : b0 + lane < a.batch ? context(a, b0 + lane) : 0; };
+    // Tokens per split.  Cut evenly: the smallest of five sizes whose splits fit the
+    // slots; the last one always does: sum ceil(len / size) <= sum len / size + batch.
+    int size = a.partition;
+    if (size == 0 && a.slots <= a.batch) size = INT32_MAX / 4 / kCut * kCut;  // a split each
+    if (size == 0) {
+        float total = 0.f;  // in units of 64 tokens, rounded up, so that 64 of them fit an integer
+        for (int b0 = 0; b0 < a.batch; b0 += kWave) total += (float)wave_sum((ctx_of(b0) + 63) / 64) * 64.f;
+        for (int spare = 0;; ++spare) {
+            const float of = fmaxf((float)a.slots - (float)a.batch * 0.25f * (float)spare, 1.f);
+            if (spare == 4) {
+                size = max(((int)fminf(total * 1.0005f / of, 0x1p29f) + kCut) / kCut * kCut, kMinSplit);
+                break;
+            }
+            size = max(((int)fminf(total / of, 0x1p29f) + kCut - 1) / kCut * kCut, kMinSplit);
+            int count = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+                const int ns = cut_context(ctx_of(b0), size, a.max_tok).ns;
+                count += wave_sum(b0 + lane < a.batch ? ns : 0);
+            }
+            if (count <= a.slots) break;
+        }
+    }
+    // Every wave counts the splits of the sequences in order.
     Segment s;
     s.b = -1;
-    const int size = split_size(a, lane);
     int before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-        const int b = b0 + lane, ctx = b < a.batch ? context(a, b) : 0;
-        const Cut c = cut_context(ctx, size);
-        int sum = b < a.batch ? c.ns : 0;  // inclusive
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const int y = __shfl_up(sum, d, kWave);
-            if (lane >= d) sum += y;
-        }
+        const int ctx = ctx_of(b0);
+        const Cut c = cut_context(ctx, size, a.max_tok);
+        const int sum = wave_inclusive_sum(b0 + lane < a.batch ? c.ns : 0);
         const uint64_t here = __builtin_amdgcn_ballot_w64(before + sum > slot);
         if (here != 0) {
             const int l = __builtin_ctzll(here);
@@ -714,17 +720,21 @@ hipError_t launch_typed(const DecodeMxArgs& x) {
 
 }  // namespace
 
-// Splits of a kv head over the whole batch.  Cut evenly: three workgroups for each
-// of the 256 CUs, or a quarter more than sequences (that the longest are cut), none
-// of less than kMinSplit tokens, and no more than 64 a sequence on average for one
-// workgroup to merge.  Measured at 256 / 512 / 768 / 1024 / 2048 workgroups, us:
-// 16 x 8192 tokens, Hq=32, Hkv=8, 4 bits 35.2 / 30.5 / 32.3 / 32.7 / 40.2; 8 x 32768,
-// 32 heads, D=64, 4 bits with weights 323 / 209 / 187 / 192 / 191; 16 of 512-8192,
+// Splits of a kv head over the whole batch.  Cut evenly: a workgroup for every 272
+// KB of K and V at max_ctx, but one to three for each of the 256 CUs; at least a
+// quarter more than sequences (that the longest are cut), none of less than
+// kMinSplit tokens, and no more than 64 a sequence on average for one workgroup to
+// merge.  Measured at 256 / 512 / 768 / 1024 / 2048 workgroups, us: 16 x 8192 tokens,
+// Hq=32, Hkv=8, 4 bits 35.2 / 30.5 / 32.3 / 32.7 / 40.2; 4 x 4096 12.3 / 14.9 / 14.8; 8 x
+// 32768, 32 heads, D=64, 4 bits with weights 323 / 209 / 187 / 192 / 191; 16 of 512-8192,
 // Hq=64, Hkv=8, fp16 with weights 85.2 / 82.9 / 82.0 / 80.8 / 83.4.
-int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition) {
+// row_bytes: of a token's K and V for one kv head.
+int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition, int64_t row_bytes) {
     if (partition > 0) return batch * ((max_ctx + partition - 1) / partition);
-    const int64_t workgroups = 768, most = 64;
-    const int64_t chunks = std::min(most, (max_ctx + kMinSplit - 1) / kMinSplit);
+    constexpr int64_t kBytes = 272 << 10, kMost = 64;
+    const double bytes = (double)batch * (double)hkv * (double)max_ctx * (double)row_bytes;
+    const int64_t workgroups = (int64_t)std::min(768.0, std::max(256.0, bytes / kBytes));
+    const int64_t chunks = std::min(kMost, (max_ctx + kMinSplit - 1) / kMinSplit);
     return std::min(batch * chunks, std::max((workgroups + hkv - 1) / hkv, batch + (batch + 3) / 4));
 }
 
