@@ -118,7 +118,7 @@ def test_page_sizes(fmt, dtype, bs):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("partition", [256, 300, 1024, 1 << 20])
 def test_splits(fmt, d, partition):
-    """Few splits, more than the decode kernel merges itself (32), one."""
+    """Few splits, many, one."""
     c = Case([9000, 1, 256, 257, 0], 1, 3, d, fmt=fmt, seed=partition)
     c.tracked(partition=partition)
     if fmt == "mxfp4":
@@ -296,3 +296,53 @@ def test_other_streams_and_repeats(fmt):
     c.check(split)
     twice = 2 * (w - c.gpu(c.weights)) + c.gpu(c.weights)
     assert torch.allclose(w2, twice, rtol=2 ** -18, atol=2 ** -20)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "full"])
+@pytest.mark.parametrize("partition", [None, 256])
+def test_more_sequences_than_lanes(fmt, partition):
+    """Splits are counted 64 sequences at a time; the longest contexts are not among the first."""
+    r = np.random.default_rng(17)
+    lens = [int(n) for n in r.integers(0, 150, 150)]
+    lens[70], lens[149], lens[64], lens[63] = 1900, 1201, 0, 600
+    c = Case(lens, 2, 2, 64, fmt=fmt, seed=17)
+    c.tracked(partition=partition)
+    if fmt == "mxfp4":
+        for _ in range(2):
+            c.check(c.run(partition=partition))
+
+
+@pytest.mark.parametrize("fmt,group", [("mxfp4", 2), ("full", 1), ("full", 9)])
+def test_weights_of_large_batches(fmt, group):
+    """Enough tokens that a thread has four of them, and more than eight heads."""
+    r = np.random.default_rng(18)
+    lens = [int(n) for n in r.integers(0, 40, 260)]
+    lens[100] = 1021
+    Case(lens, 8, group, 64, fmt=fmt, seed=18).tracked()
+
+
+def test_contexts_past_2_24():
+    """Tokens past 2^24 of one sequence, whose cut is counted in integers: 2^24 + 300 tokens on one shared page, and
+    the last 300 on their own."""
+    n, bs = (1 << 24) + 300, 1024
+    c = Case([bs, 300], 1, 2, 64, bs=bs, fmt="mxfp4", seed=19, spare=0)
+    page, last = int(c.tables[0, 0]), int(c.tables[1, 0])
+    tables = torch.full((1, -(-n // bs)), page, dtype=torch.int32, device="cuda")
+    tables[0, -1] = last
+    w = torch.zeros(1, 1, n, device="cuda")
+    q = c.gpu(c.q, torch.float16)[:1]
+    out = ak.paged_decode_mxfp4(q, *c.caches, tables, torch.tensor([n], dtype=torch.int32, device="cuda"), n, weights=w)
+    k, v = (torch.from_numpy(np.concatenate([x[page, 0], x[last, 0, :300]])) for x in c.values)
+    s = k @ torch.from_numpy(c.q[0]).T / 8
+    times = torch.ones(bs + 300).double()
+    times[:bs] = (1 << 24) // bs
+    p = torch.exp(s - s.max()) * times[:, None]
+    p = p / p.sum(0)
+    # P and the output are rounded once each (2^-11).  A wave has 2^11 tiles, so its sums take 2^11 additions one after
+    # the other, each off by a step at most (2^-12 in all).
+    assert torch.allclose(out[0].double().cpu(), p.T @ v, rtol=0,
+                          atol=(2.0 ** -10 + 2.0 ** -11) * float((p.T @ v.abs()).max()))
+    want = (p / times[:, None]).sum(1)
+    got = w[0, 0].double().cpu()
+    assert torch.allclose(got[:1 << 24].view(-1, bs), want[None, :bs].expand((1 << 24) // bs, bs), rtol=2.0 ** -11, atol=0)
+    assert torch.allclose(got[1 << 24:], want[bs:], rtol=2.0 ** -11, atol=0)

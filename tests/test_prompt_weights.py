@@ -21,9 +21,9 @@ def _check(q, k, cu, got, last=None, scale=None):
     want, reach = oracle.prompt(q.double().numpy(), k.double().numpy(), cu.tolist(), got.shape[2], last, scale)
     d = q.shape[2]
     # A score: D products in fp32 and a few roundings; a weight: its own score's and its row sum's error.  The sums over
-    # queries and heads are of positive terms, at most 2^-18 of the total at these lengths (a fp32 sum of n terms in
-    # 16-row steps is off by less than n / 16 + 20 halves of a step).
-    rel = 2 * (d + 8) * 2.0 ** -24 * (reach + 8) + 2.0 ** -18
+    # queries and heads are of positive terms: a row's sum takes up to 2500 / 32 additions one after the other, a
+    # column's 512 / 4 within a range and one for each of the ranges and heads, together under 2^8 halves of a step.
+    rel = 2 * (d + 8) * 2.0 ** -24 * (reach + 8) + 2.0 ** -16
     got = got.double().cpu().numpy()
     assert (np.abs(got - want) <= want * rel + 2.0 ** -60).all(), np.nanmax(np.abs(got - want) / (want * rel + 2.0 ** -60))
 
@@ -142,3 +142,37 @@ def test_many_ranges_and_splits_agree_with_one():
     ak.prompt_weights(q.cuda(), k.cuda(), cu2.cuda(), 2300, w2)
     _check(q, k, cu, w2[:1])
     assert not w2[1:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_prompts(dtype, d):
+    """Enough work for 64 columns a wave."""
+    lens = [2300, 1]
+    q, k, cu = _case(lens, 8, 2, d, dtype, seed=d)
+    w = torch.full((2, 2, 2305), float("nan"), device="cuda")
+    ak.prompt_weights(q.cuda(), k.cuda(), cu.cuda(), 2300, w)
+    _check(q, k, cu, w)
+
+
+@pytest.mark.parametrize("hq,hkv,last", [(16, 2, 77), (16, 16, 64), (32, 4, 5)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_prompts(hq, hkv, last, dtype):
+    """64 columns a wave for a few queries of each of 41 prompts: several heads' queries in one stream, and a stream of
+    all of them, which writes the weights itself.  max_seqlen is a bound far above the lengths."""
+    lens = [300, 0, 1, 65, 64, 63, 256, 257] + [23 + i for i in range(31)] + [0, 281]
+    q, k, cu = _case(lens, hq, hkv, 64, dtype, seed=hkv)
+    w = torch.full((41, hkv, 2500), float("nan"), device="cuda")
+    ak.prompt_weights(q.cuda(), k.cuda(), cu.cuda(), 2500, w, last=last)
+    _check(q, k, cu, w, last)
+
+
+@pytest.mark.parametrize("last", [1, 64, 512])
+def test_one_stream_writes_all_of_the_weights(last):
+    """One query head per kv head and few queries: no sums to add, and zeros behind the prompts all the same."""
+    lens = [300, 0, 129, 1]
+    q, k, cu = _case(lens, 3, 3, 128, torch.float16, seed=last)
+    big = torch.full((4, 3, 1010), float("nan"), device="cuda")
+    ak.prompt_weights(q.cuda(), k.cuda(), cu.cuda(), 300, big[:, :, :1001], last=last)
+    _check(q, k, cu, big[:, :, :1001], last)
+    assert big[:, :, 1001:].isnan().all()
