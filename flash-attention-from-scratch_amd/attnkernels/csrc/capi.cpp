@@ -226,6 +226,8 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": null pointer");
     if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": q, caches and out must be 16-byte aligned");
+    if (!aligned16(k_scales) || !aligned16(v_scales))
+        return fail(AK_ERR_INVALID_ARGUMENT, who + ": scales must be 16-byte aligned");
     for (const void* p : {(const void*)block_tables, (const void*)context_lens, (const void*)weights,
                           (const void*)counters})
         if (reinterpret_cast<uintptr_t>(p) & 3u)

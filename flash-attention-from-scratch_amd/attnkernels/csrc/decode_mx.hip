@@ -243,14 +243,51 @@ __device__ __forceinline__ uint32_t loose(uint16_t x) {
 template <int D, class T, bool MX>
 struct Tile {
     static constexpr int KW = MX ? D / 32 : D / 8;    // dwords of K per block: a quarter row
-    static constexpr int VW = MX ? 1 : D / 32;        // dwords of a V row's D/16 channels (4 bits, D = 64: half of one)
+    static constexpr int VW = MX ? D / 32 : D / 8;    // dwords of V per block: 4 bits, a quarter row; else D/16 channels of four
     // The two-byte words of D = 64 stay two bytes until they are used: widened
     // where they are loaded, the compiler would wait for them there.
     typedef std::conditional_t<MX && D == 64, uint16_t, uint32_t> word_t;
-    uint32_t k[2][KW];
-    word_t v[2][4][VW];
-    word_t ks[2], vs[2][4];  // a row's scales: 4 or 2 bytes
+    uint32_t k[2][KW], v[2][VW];
+    word_t ks[2];                     // a row's scales: 4 or 2 bytes
+    uint32_t vs[2][MX ? D / 32 : 1];  // four rows' scales
 };
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t* to, const void* from) {
+    typedef uint32_t vec __attribute__((ext_vector_type(N)));
+    const vec y = __builtin_nontemporal_load(static_cast<const vec*>(from));
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = y[i];
+}
+
+// Lane j of a quad has token j's codes, a part for each of the four lanes (a dword
+// in D = 128, half of one in D = 64); it gets its own part of all four tokens.
+template <int D>
+__device__ __forceinline__ void transpose_quad(const uint32_t (&in)[D / 32], uint32_t (&out)[D / 32], int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+    // Arguments are evaluated first: every lane takes part in the exchange.
+    auto select = [](bool which, uint32_t x, uint32_t y) { return which ? x : y; };
+    auto across1 = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, true); };
+    auto across2 = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, true); };
+    if constexpr (D == 128) {
+        uint32_t pair[4];  // tokens even, odd; parts of the lower two lanes, of the upper two
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            pair[i] = select(odd, across1(in[i + 1]), in[i]);
+            pair[i + 1] = select(odd, in[i + 1], across1(in[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            out[i] = select(high, across2(pair[i + 2]), pair[i]);
+            out[i + 2] = select(high, pair[i + 2], across2(pair[i]));
+        }
+    } else {
+        const uint32_t mine = odd ? 0x03020706u : 0x05040100u;  // (other's, own): halves of (token 0, token 1)
+        const uint32_t pair[2] = {select(high, across2(in[1]), in[0]), select(high, in[1], across2(in[0]))};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) out[i] = __builtin_amdgcn_perm(across1(pair[i]), pair[i], mine);
+    }
+}
 
 template <int D, class T, bool MX, bool WEIGHTS>
 __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) {
@@ -297,42 +334,28 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     // row.  Of the scales it loads a row's (4 or 2 bytes) and shifts its group's.
     constexpr int SROW = D / 32;
     typedef typename Tl::word_t word_t;
-    const uint32_t k_off = n * KROW + (MX ? KROW / 4 : 16) * g, v_off = 4 * g * KROW + KROW / 16 * n;
-    const uint32_t k_shift = g / (4 / SROW) * 8, v_shift = n / (16 / SROW) * 8;
+    const uint32_t k_off = n * KROW + (MX ? KROW / 4 : 16) * g;
+    // V in 16 bits: D/16 channels of rows 4g .. 4g + 3.  In 4 bits a quarter of one row,
+    // so that one load reads whole cache lines; the four lanes of a quad then trade.
+    const uint32_t v_in = MX ? n / 4 * (KROW / 4) : KROW / 16 * n, v_off = (4 * g + (MX ? n % 4 : 0)) * KROW + v_in;
+    // Right rotations that put the lane's scale where a float's exponent is: the
+    // conversions read nothing else of it.
+    const uint32_t k_turn = g / (4 / SROW) * 8 + 9, v_turn = n / (16 / SROW) * 8 + 9;
     auto load_k = [&](Tl& x, int blk, const char* p, const uint8_t* sc) {
-        if constexpr (MX && D == 128) {
-            const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.k[blk][i] = y[i];
-        } else if constexpr (MX) {
-            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
-            x.k[blk][0] = y[0];
-            x.k[blk][1] = y[1];
+        if constexpr (MX) {
+            load_words<Tl::KW>(x.k[blk], p);
         } else {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 64 * s));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x.k[blk][4 * s + i] = y[i];
-            }
+            for (int s = 0; s < KS; ++s) load_words<4>(x.k[blk] + 4 * s, p + 64 * s);
         }
         if constexpr (MX) x.ks[blk] = *reinterpret_cast<const word_t*>(sc);
     };
-    auto load_v = [&](Tl& x, int blk, int r, const char* p, const uint8_t* sc) {
-        if constexpr (MX && D == 128) {
-            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
-        } else if constexpr (MX) {
-            x.v[blk][r][0] = __builtin_nontemporal_load(reinterpret_cast<const word_t*>(p));
-        } else {
-            typedef uint32_t vec __attribute__((ext_vector_type(Tl::VW)));
-            const vec y = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p));
-#pragma unroll
-            for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = y[i];
-        }
-        if constexpr (MX) x.vs[blk][r] = *reinterpret_cast<const word_t*>(sc);
+    auto load_v = [&](Tl& x, int blk, int r, const char* p) {  // in 4 bits r is 0
+        load_words<MX ? Tl::VW : Tl::VW / 4>(x.v[blk] + r * (Tl::VW / 4), p);
     };
-    auto group_scale = [](word_t word, uint32_t shift) { return mx_scale(loose(word) >> shift & 255u); };
+    auto group_scale = [](uint32_t word, uint32_t turn) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_alignbit(word, word, turn));
+    };
     // A tile each of whose two blocks is in one page: K's or V's loads at scalar
     // bases, pa and pb the pages.
     auto load_whole = [&](Tl& x, int tile, int pa, int pb, auto what) {
@@ -346,8 +369,13 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
             const uint8_t* sbase = scales + row * SROW;
             if constexpr (V) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    load_v(x, blk, r, base + v_off + r * KROW, sbase + (uint32_t)(4 * g * SROW) + r * SROW);
+                for (int r = 0; r < (MX ? 1 : 4); ++r) load_v(x, blk, r, base + v_off + r * KROW);
+                if constexpr (MX) {
+                    typedef uint32_t vec __attribute__((ext_vector_type(SROW)));
+                    const vec y = *reinterpret_cast<const vec*>(sbase + (uint32_t)(4 * g * SROW));
+#pragma unroll
+                    for (int i = 0; i < SROW; ++i) x.vs[blk][i] = y[i];
+                }
             } else {
                 load_k(x, blk, base + k_off, sbase + (uint32_t)(n * SROW));
             }
@@ -373,15 +401,24 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
             if (valid >> (16 * blk + n) & 1)
                 load_k(x, blk, static_cast<const char*>(a.k) + kr * KROW + (k_off - n * KROW), a.k_scales + kr * SROW);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x.vs[blk][r] = 0;
+            for (int i = 0; i < Tl::VW; ++i) x.v[blk][i] = 0;
+            if constexpr (MX) {
+                const int i = 16 * blk + 4 * g + n % 4;
+                const size_t vr = row_of(i);
+                if (valid >> i & 1) load_v(x, blk, 0, static_cast<const char*>(a.v) + vr * KROW + v_in);
 #pragma unroll
-                for (int i = 0; i < Tl::VW; ++i) x.v[blk][r][i] = 0;
+                for (int i = 0; i < SROW; ++i) x.vs[blk][i] = 0;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
                 const int i = 16 * blk + 4 * g + r;
                 const size_t vr = row_of(i);
-                if (valid >> i & 1)
-                    load_v(x, blk, r, static_cast<const char*>(a.v) + vr * KROW + (v_off - 4 * g * KROW),
-                           a.v_scales + vr * SROW);
+                if (!(valid >> i & 1)) continue;
+                if constexpr (MX)
+                    x.vs[blk][r * SROW / 4] |= (uint32_t)*reinterpret_cast<const word_t*>(a.v_scales + vr * SROW)
+                                               << r * SROW % 4 * 8;
+                else
+                    load_v(x, blk, r, static_cast<const char*>(a.v) + vr * KROW + v_in);
             }
         }
         return valid;
@@ -404,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
                 u32x4 kf;
-                if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], group_scale(x.ks[blk], k_shift));
+                if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], group_scale(loose(x.ks[blk]), k_turn));
                 else kf = u32x4{x.k[blk][4 * i], x.k[blk][4 * i + 1], x.k[blk][4 * i + 2], x.k[blk][4 * i + 3]};
                 s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
             }
@@ -466,28 +503,34 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
         if constexpr (MX) {
             float sc[8];
             uint32_t v[8];
+            // Tokens 4g + r of each block, D/16 channels: a dword, in D = 64 two tokens in one.
+            uint32_t codes[2][Tl::VW];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sc[i] = group_scale(x.vs[i / 4][i % 4], v_shift);
+            for (int blk = 0; blk < 2; ++blk) transpose_quad<D>(x.v[blk], codes[blk], lane);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<0>(loose(x.v[i / 4][i % 4][0]), sc[i]);
-            channels(v, 0);
+            for (int i = 0; i < 8; ++i) sc[i] = group_scale(x.vs[i / 4][i % 4 * SROW / 4], v_turn + i % 4 * SROW % 4 * 8);
+            auto decode = [&](auto byte) {  // channels 2 byte, 2 byte + 1
+                constexpr int C = decltype(byte)::value;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<1>(loose(x.v[i / 4][i % 4][0]), sc[i]);
-            channels(v, 1);
-            if constexpr (DPL == 8) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<2>(x.v[i / 4][i % 4][0], sc[i]);
-                channels(v, 2);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = Half<T>::template decode<3>(x.v[i / 4][i % 4][0], sc[i]);
-                channels(v, 3);
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t word = codes[i / 4][i % 4 * SROW / 4];
+                    if (D == 64 && i % 2) v[i] = Half<T>::template decode<(C + 2) % 4>(word, sc[i]);
+                    else v[i] = Half<T>::template decode<C>(word, sc[i]);
+                }
+                channels(v, C);
+            };
+            decode(std::integral_constant<int, 0>{});
+            decode(std::integral_constant<int, 1>{});
+            if constexpr (D == 128) {
+                decode(std::integral_constant<int, 2>{});
+                decode(std::integral_constant<int, 3>{});
             }
         } else {
 #pragma unroll
             for (int c = 0; c < DPL / 2; ++c) {
                 uint32_t v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = x.v[i / 4][i % 4][c];
+                for (int i = 0; i < 8; ++i) v[i] = x.v[i / 4][i % 4 * (DPL / 2) + c];
                 channels(v, c);
             }
         }
