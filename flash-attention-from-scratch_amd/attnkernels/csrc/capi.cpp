@@ -237,7 +237,7 @@ int decode_mx(const char* name, const void* q, const void* k_cache, const void* 
         return fail(AK_ERR_INVALID_ARGUMENT, who + ": size out of range");
     const int64_t row_bytes = k_scales ? head_dim * 17 / 16 : 4 * head_dim;
     const int64_t slots = ak::decode_mx_slots(batch, num_kv_heads, max_context_len, partition, row_bytes);
-    if (slots > INT_MAX / num_kv_heads) return fail(AK_ERR_INVALID_ARGUMENT, who + ": too many splits");
+    if (slots > INT_MAX / num_kv_heads - 8) return fail(AK_ERR_INVALID_ARGUMENT, who + ": too many splits");
     if (weights) {
         if (w_length < max_context_len)
             return fail(AK_ERR_INVALID_ARGUMENT, who + ": weights are shorter than max_context_len");

@@ -160,6 +160,18 @@ __device__ __forceinline__ Segment segment(const Params& a, int slot, int lane) 
     return s;
 }
 
+// The kv head (x) and slot (y) of a workgroup.  Workgroups go to the eight XCDs in
+// turn.  Where there are slots for all of them, the heads of a slot go to one, whose
+// L2 then has the cache lines that hold several heads' scales of a page: 16 x 8192
+// tokens, 8 heads of 128 30.0 -> 28.9 us, 8 x 32768, 32 heads of 64 with weights
+// 657 -> 558 MB read, 157.3 -> 156.4 us.
+constexpr int kXcds = 8, kManySlots = 4 * kXcds;
+__device__ __forceinline__ int2 place_of(const Params& a, int i) {
+    if (a.slots < kManySlots) return int2{i % a.hkv, i / a.hkv};
+    const int of_xcd = i / kXcds;
+    return int2{of_xcd % a.hkv, of_xcd / a.hkv * kXcds + i % kXcds};
+}
+
 // Maximum and sum of one query row over its ns splits by 16 lanes, of which this
 // is j; every lane gets them.  Splits without weight (l = 0) count nothing; a row
 // without any has l = 0.
@@ -300,11 +312,12 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     __shared__ float red_m[kWaves][kMaxGroup], red_l[kWaves][kMaxGroup];
     __shared__ int last;
 
-    const int kvh = blockIdx.x % a.hkv;
+    const int2 place = place_of(a, blockIdx.x);
+    const int kvh = place.x;
     const int G = a.group, hq = a.hkv * G;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const Segment sg = segment(a, blockIdx.x / a.hkv, lane);
+    const Segment sg = segment(a, place.y, lane);
     if (sg.b < 0) return;
     const int b = sg.b, start = sg.split * sg.piece, end = min(sg.ctx, start + sg.piece);
     const size_t row0 = (size_t)b * hq + (size_t)kvh * G;
@@ -737,7 +750,8 @@ hipError_t launch(const DecodeMxArgs& x) {
     p.counters = WEIGHTS ? nullptr : x.counters;
     const bool finish = WEIGHTS || (x.slots > x.batch && !x.counters);
     p.cuts = finish ? static_cast<int2*>(x.cuts) : nullptr;
-    hipLaunchKernelGGL((decode_mx_kernel<D, T, MX, WEIGHTS>), dim3((unsigned)(x.hkv * x.slots)), dim3(kThreads), 0,
+    const int64_t slots = x.slots < kManySlots ? x.slots : (x.slots + kXcds - 1) / kXcds * kXcds;
+    hipLaunchKernelGGL((decode_mx_kernel<D, T, MX, WEIGHTS>), dim3((unsigned)(x.hkv * slots)), dim3(kThreads), 0,
                        (hipStream_t)x.stream, p);
     if (!finish) return hipGetLastError();
     auto run = [&](auto* kernel, int64_t workgroups) {
@@ -764,19 +778,19 @@ hipError_t launch_typed(const DecodeMxArgs& x) {
 }  // namespace
 
 // Splits of a kv head over the whole batch.  Cut evenly: a workgroup for every 272
-// KB of K and V at max_ctx, but one to three for each of the 256 CUs; at least a
+// KB of K and V at max_ctx, but one to four for each of the 256 CUs; at least a
 // quarter more than sequences (that the longest are cut), none of less than
 // kMinSplit tokens, and no more than 64 a sequence on average for one workgroup to
-// merge.  Measured at 256 / 512 / 768 / 1024 / 2048 workgroups, us: 16 x 8192 tokens,
-// Hq=32, Hkv=8, 4 bits 35.2 / 30.5 / 32.3 / 32.7 / 40.2; 4 x 4096 12.3 / 14.9 / 14.8; 8 x
-// 32768, 32 heads, D=64, 4 bits with weights 323 / 209 / 187 / 192 / 191; 16 of 512-8192,
-// Hq=64, Hkv=8, fp16 with weights 85.2 / 82.9 / 82.0 / 80.8 / 83.4.
+// merge.  Measured at 256 / 512 / 768 / 1024 / 1280 workgroups, us: 16 x 8192 tokens,
+// Hq=32, Hkv=8, 4 bits 35.2 / 30.5 / 32.3 / 32.7 / -; 4 x 4096 12.3 / 14.9 / 14.8; 8 x
+// 32768, 32 heads, D=64, 4 bits with weights - / 172 / 159 / 156 / 173; 16 of 512-8192,
+// Hq=64, Hkv=8, fp16 with weights 85.2 / 82.7 / 81.6 / 80.4 / 81.7.
 // row_bytes: of a token's K and V for one kv head.
 int64_t decode_mx_slots(int64_t batch, int64_t hkv, int64_t max_ctx, int64_t partition, int64_t row_bytes) {
     if (partition > 0) return batch * ((max_ctx + partition - 1) / partition);
     constexpr int64_t kBytes = 272 << 10, kMost = 64;
     const double bytes = (double)batch * (double)hkv * (double)max_ctx * (double)row_bytes;
-    const int64_t workgroups = (int64_t)std::min(768.0, std::max(256.0, bytes / kBytes));
+    const int64_t workgroups = (int64_t)std::min(1024.0, std::max(256.0, bytes / kBytes));
     const int64_t chunks = std::min(kMost, (max_ctx + kMinSplit - 1) / kMinSplit);
     return std::min(batch * chunks, std::max((workgroups + hkv - 1) / hkv, batch + (batch + 3) / 4));
 }
