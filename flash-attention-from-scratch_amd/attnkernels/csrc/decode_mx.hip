@@ -28,12 +28,12 @@
 // a second kernel, which knows every split's maximum and sum, turns them into
 // weights while it merges the splits' outputs.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_kernels.hpp"
 #include "index_math.hpp"
 #include "mxfp4.hpp"
 
-#include <type_traits>
 
 namespace ak {
 
@@ -272,15 +272,20 @@ __device__ __forceinline__ void load_words(uint32_t* to, const void* from) {
     for (int i = 0; i < N; ++i) to[i] = y[i];
 }
 
+// x of lanes l ^ 1, l ^ 2; as arguments of select they are evaluated by every lane.
+__device__ __forceinline__ uint32_t across1(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t across2(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t select(bool which, uint32_t x, uint32_t y) { return which ? x : y; }
+
 // Lane j of a quad has token j's codes, a part for each of the four lanes (a dword
 // in D = 128, half of one in D = 64); it gets its own part of all four tokens.
 template <int D>
 __device__ __forceinline__ void transpose_quad(const uint32_t (&in)[D / 32], uint32_t (&out)[D / 32], int lane) {
     const bool odd = lane & 1, high = lane & 2;
-    // Arguments are evaluated first: every lane takes part in the exchange.
-    auto select = [](bool which, uint32_t x, uint32_t y) { return which ? x : y; };
-    auto across1 = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, true); };
-    auto across2 = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, true); };
     if constexpr (D == 128) {
         uint32_t pair[4];  // tokens even, odd; parts of the lower two lanes, of the upper two
 #pragma unroll
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     for (int i = 0; i < KS; ++i) {
         qf[i] = u32x4{0, 0, 0, 0};
         if (n < G) {
-            const int ch = MX ? (D / 4) * g + 8 * i : 32 * i + 8 * g;
+            const int ch = MX ? (D / 4) * g + 8 * i : 64 * (i / 2) + 16 * g + 8 * (i % 2);
             qf[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + (row0 + n) * D + ch);
         }
     }
@@ -347,21 +352,24 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
     // row.  Of the scales it loads a row's (4 or 2 bytes) and shifts its group's.
     constexpr int SROW = D / 32;
     typedef typename Tl::word_t word_t;
-    const uint32_t k_off = n * KROW + (MX ? KROW / 4 : 16) * g;
-    // V in 16 bits: D/16 channels of rows 4g .. 4g + 3.  In 4 bits a quarter of one row,
-    // so that one load reads whole cache lines; the four lanes of a quad then trade.
+    // One load reads whole cache lines of 128 bytes (a second one that meets a line on
+    // its way waits for it); where those are not of the lane's own rows, lanes trade.
+    // K in 16 bits: of each line of rows n & ~1 and n | 1 the 16 bytes 2g + n % 2; lanes
+    // n and n ^ 1 trade.  V in 16 bits: D/16 channels of rows 4g .. 4g + 3.  V in 4 bits:
+    // a quarter of row 4g + n % 4; the four lanes of a quad trade.
+    constexpr int KE = MX ? 1 : 2;  // rows that a lane loads of K
+    const uint32_t k_in = MX ? KROW / 4 * g : 32 * g + 16 * (n & 1), k_off = (MX ? n : n & ~1) * KROW + k_in;
     const uint32_t v_in = MX ? n / 4 * (KROW / 4) : KROW / 16 * n, v_off = (4 * g + (MX ? n % 4 : 0)) * KROW + v_in;
     // Right rotations that put the lane's scale where a float's exponent is: the
     // conversions read nothing else of it.
     const uint32_t k_turn = g / (4 / SROW) * 8 + 9, v_turn = n / (16 / SROW) * 8 + 9;
-    auto load_k = [&](Tl& x, int blk, const char* p, const uint8_t* sc) {
+    auto load_k = [&](Tl& x, int blk, int e, const char* p) {
         if constexpr (MX) {
             load_words<Tl::KW>(x.k[blk], p);
         } else {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) load_words<4>(x.k[blk] + 4 * s, p + 64 * s);
+            for (int line = 0; line < KS / 2; ++line) load_words<4>(x.k[blk] + 4 * (2 * line + e), p + 128 * line);
         }
-        if constexpr (MX) x.ks[blk] = *reinterpret_cast<const word_t*>(sc);
     };
     auto load_v = [&](Tl& x, int blk, int r, const char* p) {  // in 4 bits r is 0
         load_words<MX ? Tl::VW : Tl::VW / 4>(x.v[blk] + r * (Tl::VW / 4), p);
@@ -390,7 +398,9 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
                     for (int i = 0; i < SROW; ++i) x.vs[blk][i] = y[i];
                 }
             } else {
-                load_k(x, blk, base + k_off, sbase + (uint32_t)(n * SROW));
+#pragma unroll
+                for (int e = 0; e < KE; ++e) load_k(x, blk, e, base + k_off + e * KROW);
+                if constexpr (MX) x.ks[blk] = *reinterpret_cast<const word_t*>(sbase + (uint32_t)(n * SROW));
             }
         }
     };
@@ -410,9 +420,14 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
             x.ks[blk] = 0;
 #pragma unroll
             for (int i = 0; i < Tl::KW; ++i) x.k[blk][i] = 0;
-            const size_t kr = row_of(16 * blk + n);
-            if (valid >> (16 * blk + n) & 1)
-                load_k(x, blk, static_cast<const char*>(a.k) + kr * KROW + (k_off - n * KROW), a.k_scales + kr * SROW);
+#pragma unroll
+            for (int e = 0; e < KE; ++e) {
+                const int i = 16 * blk + (MX ? n : (n & ~1) + e);
+                const size_t kr = row_of(i);
+                if (!(valid >> i & 1)) continue;
+                load_k(x, blk, e, static_cast<const char*>(a.k) + kr * KROW + k_in);
+                if constexpr (MX) x.ks[blk] = *reinterpret_cast<const word_t*>(a.k_scales + kr * SROW);
+            }
 #pragma unroll
             for (int i = 0; i < Tl::VW; ++i) x.v[blk][i] = 0;
             if constexpr (MX) {
@@ -451,12 +466,23 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
             s[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (MX) {
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                u32x4 kf;
-                if constexpr (MX) kf = mx_decode8<T>(x.k[blk][i], group_scale(loose(x.ks[blk]), k_turn));
-                else kf = u32x4{x.k[blk][4 * i], x.k[blk][4 * i + 1], x.k[blk][4 * i + 2], x.k[blk][4 * i + 3]};
-                s[blk] = Half<T>::mfma(kf, qf[i], s[blk]);
+                for (int i = 0; i < KS; ++i)
+                    s[blk] = Half<T>::mfma(mx_decode8<T>(x.k[blk][i], group_scale(loose(x.ks[blk]), k_turn)), qf[i], s[blk]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < KS; i += 2) {
+                    u32x4 own[2];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t even = x.k[blk][4 * i + j], odd = x.k[blk][4 * i + 4 + j];
+                        own[0][j] = select(n & 1, across1(odd), even);
+                        own[1][j] = select(n & 1, odd, across1(even));
+                    }
+                    s[blk] = Half<T>::mfma(own[0], qf[i], s[blk]);
+                    s[blk] = Half<T>::mfma(own[1], qf[i + 1], s[blk]);
+                }
             }
         }
         __builtin_amdgcn_sched_barrier(0);  // the next loads take these registers
