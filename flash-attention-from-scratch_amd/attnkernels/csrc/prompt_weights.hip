@@ -22,6 +22,7 @@
 // the first tile unless a sum passes 2^100: sums are in fp32, whose exponent has
 // room for the rest.
 #include <algorithm>
+#include <numeric>
 
 #include "attn_kernels.hpp"
 #include "mxfp4.hpp"
@@ -39,10 +40,10 @@ constexpr int kTile = 64;             // rows of a streamed tile
 constexpr int kRing = 3;              // tiles in LDS: one in use, two on their way
 constexpr int kRows = 512;            // queries whose maxima and sums a workgroup of the second pass has in LDS
 // Wave tiles from which on a wave holds 64 columns.  Measured with 64 / 32 columns,
-// us, Hq=32, Hkv=8, D=128, all queries: 512 tokens (2048 tiles) 29.1 / 23.9, 1111
-// (10368) 44.8 / 42.0, 1500 (18432) 54.3 / 49.3, 2048 (32768) 83.5 / 85.0, 8192
-// (524288) 687 / 742; 12 x 4096, the last 64 (24576) 89.5 / 95.0.
-constexpr double kManyTiles = 20000;
+// us, Hq=32, Hkv=8, D=128, all queries: 512 tokens (1024 tiles) 29.1 / 23.9, 1111
+// (5184) 44.8 / 42.0, 1500 (9216) 54.3 / 49.3, 2048 (16384) 83.5 / 85.0, 8192 (262144)
+// 687 / 742; the last 64 of 12 prompts of 1110-4096 (17700) 89.5 / 95.0.
+constexpr double kManyTiles = 14000;
 constexpr float kLowest = -3.402823466e38f;
 
 struct Params {
@@ -54,10 +55,20 @@ struct Params {
     int64_t q_stride, k_stride, w_stride_b, w_stride_h;
     int total, hkv, group, max_seqlen, last, length;
     int key_range, key_splits, heads, items_h, row_range, ranges;
+    int turn;             // sequences that a workgroup's rank among its pair's is turned by
     int held;             // keys of a workgroup of the second pass
     int pairs, key_tiles;  // (sequence, kv head) pairs, the fastest part of a workgroup's number: one's keys meet in one L2
     float sl2;
 };
+
+// The sequence of a workgroup.  An XCD's workgroups go to its four shader engines in
+// turn, so one sequence's would all be on one of them where batch * hkv is a multiple
+// of 32: the sequences take turns too, by a.turn, which keeps a pair on its XCD.  The
+// last 64 queries of 12 prompts of 1110-4096 tokens, Hkv=8: first pass 46.5 -> 36.3 us.
+__device__ __forceinline__ int batch_of(const Params& a, int pair, int index) {
+    const int batch = a.pairs / a.hkv;
+    return (pair / a.hkv + index % batch * a.turn) % batch;
+}
 
 struct Sequence {
     int start, n, first;  // rows in the packed tensors, tokens, first query that counts
@@ -180,14 +191,15 @@ __device__ __forceinline__ int row_of(int r, int lane) { return 8 * (r / 4) + 4 
 template <int D, class T, int C>
 __global__ void __launch_bounds__(kThreads, C == 2 ? 2 : 3) prompt_stats_kernel(const Params a) {
     __shared__ u32x4 tiles[kRing][kTile * kUnits<D>];
-    const int pair = blockIdx.x % a.pairs, kvh = pair % a.hkv, b = pair / a.hkv;
+    const int pair = blockIdx.x % a.pairs, kvh = pair % a.hkv, index = blockIdx.x / a.pairs;
+    const int b = batch_of(a, pair, index);
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int G = a.group;
     const Sequence sq = sequence(a, b);
     const int R = sq.n - sq.first;
     const int chunks = (R + kCols<C> - 1) / kCols<C> * G;
     // The longest streams first: the last queries have the lowest workgroup numbers.
-    const int groups = (chunks + kWaves - 1) / kWaves, index = blockIdx.x / a.pairs;
+    const int groups = (chunks + kWaves - 1) / kWaves;
     const int part = index % a.key_splits, group = groups - 1 - index / a.key_splits;
     if (group < 0) return;
     const int chunk = min(group * kWaves + w, chunks - 1);
@@ -302,8 +314,9 @@ __global__ void __launch_bounds__(kThreads, C == 2 ? 2 : 3) prompt_sums_kernel(c
     __shared__ u32x4 tiles[kRing][kTile * kUnits<D>];
     __shared__ f32x4 row_m[kRows / 4], row_w[kRows / 4];
     // The last ranges, which all keys stream, first.
-    const int pair = blockIdx.x % a.pairs, kvh = pair % a.hkv, b = pair / a.hkv;
+    const int pair = blockIdx.x % a.pairs, kvh = pair % a.hkv;
     int index = blockIdx.x / a.pairs;
+    const int b = batch_of(a, pair, index);
     const int part = index % a.items_h, head0 = part * a.heads;
     index /= a.items_h;
     const int kt = index % a.key_tiles, j = a.ranges - 1 - index / a.key_tiles, item = part * a.ranges + j;
@@ -451,18 +464,23 @@ struct Plan {
     int64_t key_tiles, stats_workgroups, sums_workgroups;
 };
 
-Plan make_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t max_seqlen, int64_t last, int64_t length) {
+Plan make_plan(int64_t batch, int64_t total, int64_t hq, int64_t hkv, int64_t max_seqlen, int64_t last,
+               int64_t length) {
     Plan p;
     const int64_t rows = std::min(last, max_seqlen), group = hq / hkv, pairs = batch * hkv;
+    // Prompts of max_seqlen that hold as many tokens as there are.
+    const double full = std::min((double)batch, (double)total / (double)max_seqlen);
     auto groups_of = [&](int64_t columns) {
         return ((rows + 32 * columns - 1) / (32 * columns) * group + kWaves - 1) / kWaves;
     };
-    // Wave tiles of 64 columns and 64 rows, counted as if no mask cut them.
-    const double tiles = (double)batch * hq * ((rows + 63) / 64) * ((max_seqlen + 63) / 64);
+    // Wave tiles of 64 columns and 64 rows.
+    const double r = (double)((rows + 63) / 64), tiles = full * (double)hq * r * ((double)((max_seqlen + 63) / 64) - r / 2);
     p.columns = tiles >= kManyTiles ? 2 : 1;
     const int64_t slots = p.columns == 2 ? 512 : 768, groups = groups_of(p.columns);
     const int64_t most = (max_seqlen + 127) / 128;  // ranges of at least 128 keys
-    const int64_t want = std::max<int64_t>(1, std::min(most, slots / std::max<int64_t>(1, groups * pairs)));
+    // A sequence's last split is half empty on average.
+    const double spare = (double)slots - 0.5 * (double)(groups * pairs);
+    const int64_t want = std::max<int64_t>(1, std::min(most, (int64_t)(spare / (full * (double)(groups * hkv)))));
     p.key_range = ((max_seqlen + want - 1) / want + kTile - 1) / kTile * kTile;
     p.key_splits = (max_seqlen + p.key_range - 1) / p.key_range;
     p.row_range = kRows;
@@ -512,6 +530,8 @@ hipError_t launch(const PromptWeightsArgs& x, const Plan& plan) {
     p.row_range = (int)plan.row_range;
     p.ranges = (int)plan.ranges;
     p.sl2 = x.sl2;
+    const int step = 8 / std::gcd(8, (int)x.hkv);
+    p.turn = x.batch % step == 0 ? step : 0;
     p.held = kHeld<C>;
     p.pairs = (int)(x.batch * x.hkv);
     p.key_tiles = (int)plan.key_tiles;
@@ -528,7 +548,7 @@ hipError_t launch(const PromptWeightsArgs& x, const Plan& plan) {
 
 template <int D, class T>
 hipError_t launch_columns(const PromptWeightsArgs& x) {
-    const Plan plan = make_plan(x.batch, x.hq, x.hkv, x.max_seqlen, x.last, x.length);
+    const Plan plan = make_plan(x.batch, x.total, x.hq, x.hkv, x.max_seqlen, x.last, x.length);
     return plan.columns == 2 ? launch<D, T, 2>(x, plan) : launch<D, T, 1>(x, plan);
 }
 
@@ -536,7 +556,7 @@ hipError_t launch_columns(const PromptWeightsArgs& x) {
 
 size_t prompt_weights_workspace(int64_t batch, int64_t total, int64_t hq, int64_t hkv, int64_t max_seqlen,
                                 int64_t last) {
-    const Plan p = make_plan(batch, hq, hkv, max_seqlen, last, max_seqlen);
+    const Plan p = make_plan(batch, total, hq, hkv, max_seqlen, last, max_seqlen);
     return sizeof(float) * (size_t)total * (size_t)(2 * p.key_splits * hq + hkv * p.items_h * p.ranges);
 }
 
@@ -559,7 +579,7 @@ hipError_t prompt_weights_launch(const PromptWeightsArgs& x) {
 
 bool prompt_weights_fits(const PromptWeightsArgs& x) {
     if (x.total == 0 || x.max_seqlen == 0) return true;
-    const Plan p = make_plan(x.batch, x.hq, x.hkv, x.max_seqlen, x.last, x.length);
+    const Plan p = make_plan(x.batch, x.total, x.hq, x.hkv, x.max_seqlen, x.last, x.length);
     return std::max(p.stats_workgroups, p.sums_workgroups) <= INT32_MAX;
 }
 

@@ -148,22 +148,22 @@ def test_many_ranges_and_splits_agree_with_one():
 @pytest.mark.parametrize("d", [64, 128])
 def test_long_prompts(dtype, d):
     """Enough work for 64 columns a wave."""
-    lens = [2300, 1]
-    q, k, cu = _case(lens, 8, 2, d, dtype, seed=d)
-    w = torch.full((2, 2, 2305), float("nan"), device="cuda")
-    ak.prompt_weights(q.cuda(), k.cuda(), cu.cuda(), 2300, w)
+    lens = [2000, 1]
+    q, k, cu = _case(lens, 32, 2, d, dtype, seed=d)
+    w = torch.full((2, 2, 2005), float("nan"), device="cuda")
+    ak.prompt_weights(q.cuda(), k.cuda(), cu.cuda(), 2000, w)
     _check(q, k, cu, w)
 
 
-@pytest.mark.parametrize("hq,hkv,last", [(16, 2, 77), (16, 16, 64), (32, 4, 5)])
+@pytest.mark.parametrize("hq,hkv,last", [(64, 8, 77), (64, 64, 100), (64, 16, 128)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_many_prompts(hq, hkv, last, dtype):
     """64 columns a wave for a few queries of each of 41 prompts: several heads' queries in one stream, and a stream of
     all of them, which writes the weights itself.  max_seqlen is a bound far above the lengths."""
-    lens = [300, 0, 1, 65, 64, 63, 256, 257] + [23 + i for i in range(31)] + [0, 281]
+    lens = [300, 0, 1, 65, 64, 63, 256, 257] + [123 + 6 * i for i in range(31)] + [0, 281]
     q, k, cu = _case(lens, hq, hkv, 64, dtype, seed=hkv)
     w = torch.full((41, hkv, 2500), float("nan"), device="cuda")
-    ak.prompt_weights(q.cuda(), k.cuda(), cu.cuda(), 2500, w, last=last)
+    ak.prompt_weights(q.cuda(), k.cuda(), cu.cuda(), 1000, w, last=last)
     _check(q, k, cu, w, last)
 
 
