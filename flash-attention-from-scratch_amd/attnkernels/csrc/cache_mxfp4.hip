@@ -10,7 +10,10 @@
 // holds 8 channels (16 bytes, 4 bytes of codes), so four lanes are a scale
 // group: its largest magnitude comes from two DPP lane exchanges on the bit
 // patterns (magnitudes of one type order as integers), and the codes from the
-// hardware's conversions, which round to nearest even.
+// hardware's conversions, which round to nearest even.  Rows of the wide side are
+// read and written once, 16 bytes a lane.  Measured: 16384 tokens, 8 heads of 128 from
+// a fused projection 18.6 us to write (4.6 TB/s) and 17.5 to read back (4.9 TB/s; a
+// copy reaches 4.9); 64 tokens 4.5 us each, the launch and two round trips.
 #include <hip/hip_runtime.h>
 
 #include "attn_kernels.hpp"

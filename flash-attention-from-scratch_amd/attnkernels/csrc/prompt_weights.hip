@@ -21,6 +21,11 @@
 // exponentials a score.  The maximum subtracted in the first pass is the one of
 // the first tile unless a sum passes 2^100: sums are in fp32, whose exponent has
 // room for the rest.
+// A stage's products run beside the exponentials of the block before.  Measured,
+// Hq=32, Hkv=8, D=128: 8192 tokens, all queries, about 670 us (the two passes 0.82
+// PFLOP/s), 2.8 us a tile of 64 rows where two workgroups share a CU; the products
+// alone are 1.0, the vector work alone 1.1, both with nothing to wait for 1.6; 1111 tokens 41 us (19 + 19 + 3, a chain
+// of few tiles a workgroup); the last 64 queries of 12 prompts of 1110-4096 tokens 70.
 #include <algorithm>
 #include <numeric>
 

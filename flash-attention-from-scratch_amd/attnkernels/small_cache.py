@@ -53,6 +53,8 @@ def paged_decode_mxfp4(q, k_cache, k_scales, v_cache, v_scales, block_tables, co
 
     q:            [B, H, D] fp16 or bf16, D in {64, 128}, H / H_kv from 1 to 16; the
                   cache's values are rounded to its type
+    k_cache, k_scales, v_cache, v_scales: 16-byte aligned (whole tensors and slices
+                  of whole pages of 16 tokens are)
     block_tables, context_lens, max_context_len, scale: as in paged_decode; a
                   context of 0 tokens gives zeros, tokens from max_context_len on
                   are ignored

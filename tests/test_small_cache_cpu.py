@@ -253,6 +253,10 @@ def _decode(lib, weights=FAKE, full=False, **over):
                                      a["ncount"], None)
 
 
+def test_capi_decode_refuses_misaligned_scales(lib):
+    _refused(lib, _decode(lib, ks=FAKE + 2), 1, "scales must be 16-byte aligned")
+
+
 @pytest.mark.parametrize("code,word,over", [
     (1, "multiple of num_kv_heads", dict(hq=5)), (1, "positive multiple of 256", dict(part=100)), (1, "positive multiple of 256", dict(part=-256)),
     (2, "at most 16", dict(hq=34)), (2, "head_dim", dict(d=32)), (1, "invalid size", dict(bs=0)),
