@@ -361,20 +361,21 @@ __global__ void __launch_bounds__(kThreads, C == 2 ? 2 : 3) prompt_sums_kernel(c
             const size_t at = (size_t)(h0 + head) * a.total + sq.start + pos;
             float L = 0.f;
             m = kLowest;
-            for (int p0 = 0; p0 < a.key_splits; p0 += 4) {
-                float lp[4], mp[4];
+            constexpr int kTogether = 8;  // splits whose loads are on their way together
+            for (int p0 = 0; p0 < a.key_splits; p0 += kTogether) {
+                float lp[kTogether] = {}, mp[kTogether] = {};
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {  // the loads of four splits together
-                    const size_t from = at + min(p0 + p, a.key_splits - 1) * step;
-                    lp[p] = p0 + p < a.key_splits ? a.l[from] : 0.f;
-                    mp[p] = a.m[from];
-                }
+                for (int p = 0; p < kTogether; ++p)
+                    if (p0 + p < a.key_splits) {
+                        lp[p] = a.l[at + (p0 + p) * step];
+                        mp[p] = a.m[at + (p0 + p) * step];
+                    }
                 float mx = m;
 #pragma unroll
-                for (int p = 0; p < 4; ++p) mx = lp[p] == 0.f ? mx : fmaxf(mx, mp[p]);
+                for (int p = 0; p < kTogether; ++p) mx = lp[p] == 0.f ? mx : fmaxf(mx, mp[p]);
                 L *= exp2_fast(m - mx);
 #pragma unroll
-                for (int p = 0; p < 4; ++p) L += lp[p] == 0.f ? 0.f : lp[p] * exp2_fast(mp[p] - mx);
+                for (int p = 0; p < kTogether; ++p) L += lp[p] == 0.f ? 0.f : lp[p] * exp2_fast(mp[p] - mx);
                 m = mx;
             }
             wgt = L == 0.f ? 0.f : 1.f / L;  // every score -inf: nothing
