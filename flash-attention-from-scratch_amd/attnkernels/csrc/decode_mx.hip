@@ -284,33 +284,16 @@ __device__ __forceinline__ void load_words(uint32_t* to, const void* from) {
     for (int i = 0; i < N; ++i) to[i] = y[i];
 }
 
-// x of lanes l ^ 1, l ^ 2; as arguments of select they are evaluated by every lane.
-__device__ __forceinline__ uint32_t across1(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, true);
-}
-__device__ __forceinline__ uint32_t across2(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, true);
-}
-__device__ __forceinline__ uint32_t select(bool which, uint32_t x, uint32_t y) { return which ? x : y; }
-
 // Lane j of a quad has token j's codes, a part for each of the four lanes (a dword
 // in D = 128, half of one in D = 64); it gets its own part of all four tokens.
 template <int D>
-__device__ __forceinline__ void transpose_quad(const uint32_t (&in)[D / 32], uint32_t (&out)[D / 32], int lane) {
-    const bool odd = lane & 1, high = lane & 2;
+__device__ __forceinline__ void own_codes(const uint32_t (&in)[D / 32], uint32_t (&out)[D / 32], int lane) {
     if constexpr (D == 128) {
-        uint32_t pair[4];  // tokens even, odd; parts of the lower two lanes, of the upper two
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            pair[i] = select(odd, across1(in[i + 1]), in[i]);
-            pair[i + 1] = select(odd, in[i + 1], across1(in[i]));
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            out[i] = select(high, across2(pair[i + 2]), pair[i]);
-            out[i + 2] = select(high, pair[i + 2], across2(pair[i]));
-        }
+        for (int i = 0; i < 4; ++i) out[i] = in[i];
+        transpose_quad(out[0], out[1], out[2], out[3], lane);
     } else {
+        const bool odd = lane & 1, high = lane & 2;
         const uint32_t mine = odd ? 0x03020706u : 0x05040100u;  // (other's, own): halves of (token 0, token 1)
         const uint32_t pair[2] = {select(high, across2(in[1]), in[0]), select(high, in[1], across2(in[0]))};
 #pragma unroll
@@ -557,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mx_kernel(const Params a) 
             // Tokens 4g + r of each block, D/16 channels: a dword, in D = 64 two tokens in one.
             uint32_t codes[2][Tl::VW];
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk) transpose_quad<D>(x.v[blk], codes[blk], lane);
+            for (int blk = 0; blk < 2; ++blk) own_codes<D>(x.v[blk], codes[blk], lane);
 #pragma unroll
             for (int i = 0; i < 8; ++i) sc[i] = group_scale(x.vs[i / 4][i % 4 * SROW / 4], v_turn + i % 4 * SROW % 4 * 8);
             auto decode = [&](auto byte) {  // channels 2 byte, 2 byte + 1

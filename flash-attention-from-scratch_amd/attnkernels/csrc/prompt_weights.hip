@@ -179,15 +179,34 @@ __device__ __forceinline__ void product(const u32x4* tile, int blk, const u32x4 
     }
 }
 
+// Starts the held columns' loads: rows i0 .. of `rows`, those past `end` as row end - 1.
+// A product's operand is 16 of every 32 bytes of a lane's row; loaded so, four loads
+// would meet each cache line, and all but the first would wait for it.  Instead a
+// quad's lanes load each of their four rows' lines in turn, and trade in held_ready.
 template <int D, int C>
 __device__ __forceinline__ void hold(const Rows& rows, int i0, int end, int lane, u32x4 (&held)[C][D / 16]) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int i = min(i0 + 32 * c + (lane & 31), end - 1);
+    for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-            held[c][k] = *reinterpret_cast<const u32x4*>(rows.p + i * rows.stride + 16 * k + 8 * (lane >> 5));
-    }
+        for (int k = 0; k < D / 16; ++k) {
+            const int i = min(i0 + 32 * c + (lane & 28) + k % 4, end - 1), of_line = lane & 3;
+            held[c][k] = *reinterpret_cast<const u32x4*>(rows.p + i * rows.stride + 16 * (k / 4 * 4 + of_line) +
+                                                         8 * (lane >> 5));
+        }
+}
+template <int D, int C>
+__device__ __forceinline__ void held_ready(u32x4 (&held)[C][D / 16], int lane) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < D / 16; k += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t x[4] = {held[c][k][i], held[c][k + 1][i], held[c][k + 2][i], held[c][k + 3][i]};
+                transpose_quad(x[0], x[1], x[2], x[3], lane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) held[c][k + j][i] = x[j];
+            }
 }
 
 // The row of register r of a 32 x 32 product in this lane.
@@ -282,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, C == 2 ? 2 : 3) prompt_stats_kernel(
         }
         live = now;
     };
+    held_ready<D, C>(held, lane);
     f32x16 x[C], y[C];
     for (int t = 0, cur = 0; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
         const int k0 = begin + t * kTile;
@@ -421,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, C == 2 ? 2 : 3) prompt_sums_kernel(c
         }
         live = now;
     };
+    held_ready<D, C>(held, lane);
     f32x16 x[C], y[C];
     for (int t = 0, cur = 0, i0 = begin; t < count; ++t, cur = cur == kRing - 1 ? 0 : cur + 1) {
         tile_ready<D>(count - 1 - t);

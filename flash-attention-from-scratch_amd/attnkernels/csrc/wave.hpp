@@ -114,4 +114,24 @@ __device__ __forceinline__ int xcd_chunk_remap(int bid, int total, int chunk) {
     return slot / chunk * group + x * chunk + slot % chunk;
 }
 
+// x of lanes l ^ 1, l ^ 2; as arguments of select they are evaluated by every lane.
+__device__ __forceinline__ uint32_t across1(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t across2(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t select(bool which, uint32_t x, uint32_t y) { return which ? x : y; }
+
+// Lane j of a quad gets in x[i] what lane i had in x[j].
+__device__ __forceinline__ void transpose_quad(uint32_t& x0, uint32_t& x1, uint32_t& x2, uint32_t& x3, int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+    const uint32_t a0 = select(odd, across1(x1), x0), a1 = select(odd, x1, across1(x0));
+    const uint32_t a2 = select(odd, across1(x3), x2), a3 = select(odd, x3, across1(x2));
+    x0 = select(high, across2(a2), a0);
+    x1 = select(high, across2(a3), a1);
+    x2 = select(high, a2, across2(a0));
+    x3 = select(high, a3, across2(a1));
+}
+
 }  // namespace ak
