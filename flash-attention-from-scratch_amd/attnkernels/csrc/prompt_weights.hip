@@ -24,8 +24,8 @@
 // A stage's products run beside the exponentials of the block before.  Measured,
 // Hq=32, Hkv=8, D=128: 8192 tokens, all queries, about 670 us (the two passes 0.82
 // PFLOP/s), 2.8 us a tile of 64 rows where two workgroups share a CU; the products
-// alone are 1.0, the vector work alone 1.1, both with nothing to wait for 1.6; 1111 tokens 41 us (19 + 19 + 3, a chain
-// of few tiles a workgroup); the last 64 queries of 12 prompts of 1110-4096 tokens 70.
+// alone are 1.0, the vector work alone 1.1, both with nothing to wait for 1.6; 1111 tokens 40 us (19 + 19 + 3, a chain
+// of few tiles a workgroup); the last 64 queries of 12 prompts of 1110-4096 tokens 66.
 #include <algorithm>
 #include <numeric>
 
@@ -182,7 +182,8 @@ __device__ __forceinline__ void product(const u32x4* tile, int blk, const u32x4 
 // Starts the held columns' loads: rows i0 .. of `rows`, those past `end` as row end - 1.
 // A product's operand is 16 of every 32 bytes of a lane's row; loaded so, four loads
 // would meet each cache line, and all but the first would wait for it.  Instead a
-// quad's lanes load each of their four rows' lines in turn, and trade in held_ready.
+// quad's lanes load each of their four rows' lines in turn, and trade in held_ready:
+// the last 64 queries of 12 prompts of 1110-4096 tokens 68.6 -> 66.1 us.
 template <int D, int C>
 __device__ __forceinline__ void hold(const Rows& rows, int i0, int end, int lane, u32x4 (&held)[C][D / 16]) {
 #pragma unroll

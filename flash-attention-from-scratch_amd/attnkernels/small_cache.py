@@ -115,9 +115,10 @@ def evict_cache(k_cache, v_cache, block_tables, context_lens, weights, budget, r
                   ``paged_decode_weights`` and ``prompt_weights``
     new_block_tables: None: the kept rows move to the front of the sequence's own
                   pages, and rows past them stay as they are; a page must not be in
-                  two sequences then, if one of them is cut.  Else [B,
-                  new_max_blocks] pages that all kept rows are written to (also of
-                  sequences that keep everything), none of them in block_tables
+                  two sequences then, if one of them is cut, nor twice in that one.
+                  Else [B, new_max_blocks] pages that all kept rows are written to
+                  (also of sequences that keep everything), none of them in
+                  block_tables or there twice
 
     Returns (context_lens, weights, kept): the new lengths, int32 [B]; the kept
     tokens' weights, zero past them, in new memory of the old shape; and int32

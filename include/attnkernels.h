@@ -307,7 +307,7 @@ int ak_prompt_weights(const void *q, const void *k, const int32_t *cu_seqlens, f
  *                k_scales, v_scales rows of scale_bytes bytes, or NULL and 0
  *   new_block_tables  NULL: row i of a sequence's pages becomes what row kept[i]
  *                was, rows from new_lens on stay; then no page may be in two
- *                sequences of which one is cut.  Else int32 [batch,
+ *                sequences of which one is cut, or twice in one.  Else int32 [batch,
  *                new_max_blocks]: all kept rows are written to these pages, none
  *                of which may be in block_tables or there twice.
  * Tokens past weights_length or the block table's row are ignored; rows on page
